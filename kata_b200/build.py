@@ -11,7 +11,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libkata_attn.so")
-SOURCES = ["ctx.cu", "tmap.cu", "prep.cu", "decode_scalar.cu", "decode_mma.cu", "prefill_mma.cu", "prefill_tc5.cu", "draft_attn.cu", "peer_merge.cu", "attn_engine.cpp", "kv_ckpt.cpp", "host_step.cpp"]
+SOURCES = ["ctx.cu", "tmap.cu", "prep.cu", "decode_scalar.cu", "decode_mma.cu", "prefill_mma.cu", "prefill_tc5.cu", "draft_attn.cu", "peer_merge.cu", "page_pool.cpp", "paged_ctx.cu", "paged_prep.cu", "paged_decode.cu", "paged_evict.cu", "attn_engine.cpp", "kv_ckpt.cpp", "host_step.cpp"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
               "--expt-relaxed-constexpr", "-Xptxas", "-v"]
 
@@ -27,7 +27,7 @@ def needs_build() -> bool:
     if not os.path.exists(LIB):
         return True
     t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", h) for h in ("kata_attn.h", "kata_draft.h", "kata_ckpt.h")] + [os.path.abspath(__file__)]
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", h) for h in ("kata_attn.h", "kata_draft.h", "kata_ckpt.h", "kata_engine.h", "kata_paged.h")] + [os.path.abspath(__file__)]
     return any(os.path.getmtime(d) > t for d in deps)
 
 

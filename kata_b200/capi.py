@@ -61,7 +61,7 @@ def lib() -> C.CDLL:
         L.kata_attn_kv_plane_row_bytes.restype = C.c_size_t
         L.kata_attn_kv_plane_ptr.restype = C.c_void_p
         L.kata_attn_launch_count.restype = C.c_uint64
-        for name in EXPORTS:
+        for name in EXPORTS + PAGED_EXPORTS:
             getattr(L, name)
         _lib = L
     return _lib
@@ -418,3 +418,175 @@ class PeerExchange:
         if self.h:
             self.L.kata_attn_peer_destroy(self.h)
             self.h = C.c_void_p()
+
+
+PAGED_EXPORTS = [
+    "kata_pages_create", "kata_pages_destroy", "kata_pages_reserve", "kata_pages_trim", "kata_pages_fork", "kata_pages_count", "kata_pages_get", "kata_pages_free_count", "kata_pages_owners",
+    "kata_paged_create", "kata_paged_destroy", "kata_paged_last_error", "kata_paged_launch_count", "kata_paged_check", "kata_paged_plane_ptr", "kata_paged_reserve", "kata_paged_trim", "kata_paged_fork",
+    "kata_paged_table", "kata_paged_prep", "kata_paged_decode", "kata_paged_evict", "kata_paged_import", "kata_paged_decode_plan",
+]
+_PLANES = ("k", "v", "k_scale", "v_scale", "weight", "age")   # KATA_PAGED_* planes
+PAGED_GATED, PAGED_WEIGHTS = 1, 2
+
+
+class PagedConfig(C.Structure):
+    _fields_ = [("device", C.c_int32), ("n_layers", C.c_int32), ("n_seqs", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32), ("max_slots", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("kv_mode", C.c_int32), ("rot_dim", C.c_int32), ("section", C.c_int32 * 3), ("interleaved", C.c_int32), ("flags", C.c_int32), ("rope_theta", C.c_double), ("planes", C.c_void_p * 6)]
+
+
+class PagedContext:
+    """A KV cache in pages (include/kata_paged.h): page tables, the prep that appends with positions of up to three axes, attention of
+    the newest tokens over the pages, and eviction by accumulated attention weight."""
+
+    def __init__(self, n_layers: int, n_seqs: int, n_pages: int, page_size: int, max_slots: int, heads: int = 24, kv_heads: int = 4, head_dim: int = 256, kv_mode: str = "fp16", rot_dim: int = 64, theta: float = 1e7,
+                 sections=None, interleaved: bool = False, gated: bool = True, weights: bool = False, planes=None, device: int | None = None):
+        """``sections``: rotary frequencies per axis (time, height, width), all on the first axis by default. ``planes``: the caller's tensors for planes
+        ("k", "v", "k_scale", "v_scale", "weight", "age") in the header's layout, [n_layers] of them; the others are allocated, zero-filled."""
+        L = self.L = lib()
+        L.kata_paged_last_error.restype = C.c_char_p
+        L.kata_paged_launch_count.restype = C.c_uint64
+        L.kata_paged_plane_ptr.restype = L.kata_paged_table.restype = C.c_void_p
+        self.device = torch.cuda.current_device() if device is None else device
+        self.n_layers, self.n_seqs, self.n_pages, self.page_size, self.max_slots = n_layers, n_seqs, n_pages, page_size, max_slots
+        self.heads, self.kv_heads, self.head_dim, self.kv_mode, self.gated, self.weights = heads, kv_heads, head_dim, kv_mode, gated, weights
+        if kv_mode not in _KV_MODES:
+            raise ValueError(f"kv_mode {kv_mode!r}: fp16 or int8")
+        self.planes = dict(planes or {})   # kept alive: the context works on them
+        for name, t in self.planes.items():
+            if name not in _PLANES:
+                raise ValueError(f"plane {name!r}: one of {_PLANES}")
+            want = {"k": torch.int8 if kv_mode == "int8" else torch.float16, "weight": torch.float32, "age": torch.int32}.get("k" if name == "v" else name, torch.float16)
+            n = n_layers * n_pages * page_size * kv_heads * (head_dim if name in ("k", "v") else 1)
+            if not t.is_cuda or not t.is_contiguous() or t.dtype != want or t.numel() != n or t.device.index != self.device:
+                raise ValueError(f"plane {name!r}: a contiguous {want} tensor of {n} elements on device {self.device}")
+        sec = tuple(sections) if sections is not None else (rot_dim // 2, 0, 0)
+        cfg = PagedConfig(self.device, n_layers, n_seqs, n_pages, page_size, max_slots, heads, kv_heads, head_dim, _KV_MODES[kv_mode], rot_dim, (C.c_int32 * 3)(*sec), int(interleaved),
+                          (PAGED_GATED if gated else 0) | (PAGED_WEIGHTS if weights else 0), theta, (C.c_void_p * 6)(*[self.planes[p].data_ptr() if p in self.planes else None for p in _PLANES]))
+        self.h = C.c_void_p()
+        rc = L.kata_paged_create(C.byref(cfg), C.byref(self.h))
+        if rc != OK:
+            raise KataError(rc, "kata_paged_create failed")
+
+    def close(self):
+        if self.h:
+            self.L.kata_paged_destroy(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _ck(self, rc):
+        if rc != OK:
+            raise KataError(rc, self.L.kata_paged_last_error(self.h).decode())
+
+    def _s(self):
+        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)   # the context's device, whichever is current
+
+    def check(self):
+        self._ck(self.L.kata_paged_check(self.h, self._s()))
+
+    def launches(self) -> int:
+        return int(self.L.kata_paged_launch_count(self.h))
+
+    # ---- pages
+    def reserve(self, seq: int, n_slots: int):
+        self._ck(self.L.kata_paged_reserve(self.h, seq, n_slots, self._s()))
+
+    def trim(self, seq: int, n_slots: int = 0):
+        self._ck(self.L.kata_paged_trim(self.h, seq, n_slots))
+
+    def fork(self, src: int, dst: int, n_slots: int):
+        self._ck(self.L.kata_paged_fork(self.h, src, dst, n_slots, self._s()))
+
+    def pages(self, seq: int) -> list:
+        t = C.c_void_p(self.L.kata_paged_table(self.h))
+        n = self.L.kata_pages_count(t, seq)
+        if n < 0:
+            raise KataError(2, f"sequence id {seq}")
+        buf = (C.c_int32 * max(1, n))()
+        self.L.kata_pages_get(t, seq, buf, n)
+        return list(buf)[:n]
+
+    def free_pages(self) -> int:
+        return int(self.L.kata_pages_free_count(C.c_void_p(self.L.kata_paged_table(self.h))))
+
+    def plane(self, layer: int, name: str) -> torch.Tensor:
+        """A layer's plane as a tensor that aliases it: k, v [pages][page_size][kv_heads][head_dim], scales [pages][page_size][kv_heads], weight and age [pages][kv_heads][page_size]."""
+        P, S, H, D = self.n_pages, self.page_size, self.kv_heads, self.head_dim
+        kv = name in ("k", "v")
+        shape = (P, S, H, D) if kv else (P, S, H) if name.endswith("scale") else (P, H, S)
+        if name in self.planes:
+            return self.planes[name].view(self.n_layers, *shape)[layer]
+        ptr = self.L.kata_paged_plane_ptr(self.h, layer, _PLANES.index(name))
+        if not ptr:
+            raise KataError(3, f"no plane {name!r}")
+        kind = ("|i1" if self.kv_mode == "int8" else "<f2") if kv else {"weight": "<f4", "age": "<i4"}.get(name, "<f2")
+
+        class _Alias:
+            __cuda_array_interface__ = {"shape": shape, "typestr": kind, "data": (ptr, False), "version": 3, "strides": None}
+        return torch.as_tensor(_Alias(), device=torch.device("cuda", self.device))
+
+    # ---- the operators
+    def _rows(self, what, t, shape, dtypes):
+        """A device tensor of this shape (any grouping of it) and one of these types, contiguous; raises otherwise."""
+        n = 1
+        for x in shape:
+            n *= x
+        if t.dtype not in dtypes or t.numel() != n or not t.is_cuda or t.device.index != self.device or not t.is_contiguous():
+            raise ValueError(f"{what}: a contiguous tensor {list(shape)} of {dtypes} on device {self.device} is needed, not {list(t.shape)} of {t.dtype} on {t.device}")
+        return C.c_void_p(t.data_ptr())
+
+    def prep(self, layer, seq_ids, slot0, T, q, k, v, qnorm, knorm, axis_pos=None, age0=None, q16=None, gate=None):
+        """Norm, rotary positions and append of T tokens per sequence into slots slot0.. (kata_paged_prep). q [n][T][heads][(2) head_dim] or None, k, v [n][T][kv_heads][head_dim], axis_pos int32
+        [n][T][3] or None (text: age0 + t on every axis). Returns (q16, None, gate) as AttnContext.prep does."""
+        sa, sp = _i32(seq_ids); la, lp = _i32(slot0)
+        n, H, KH, D = len(sa), self.heads, self.kv_heads, self.head_dim
+        if len(la) != n or (age0 is not None and len(age0) != n):
+            raise ValueError("one slot0 (and age0) per sequence")
+        act = (k.dtype,) if k.dtype in _ACT else tuple(_ACT)
+        kp, vp = self._rows("k", k, (n, T, KH, D), act), self._rows("v", v, (n, T, KH, D), act)
+        qp = gp = hp = C.c_void_p(0)
+        if q is not None:
+            qp = self._rows("q", q, (n, T, H, D * (2 if self.gated else 1)), act)
+            q16 = torch.empty((n, T, H * D), dtype=torch.float16, device=k.device) if q16 is None else q16
+            gate = torch.empty((n, T, H * D), dtype=torch.float32, device=k.device) if gate is None and self.gated else gate
+            hp = self._rows("q16", q16, (n, T, H, D), (torch.float16,))
+        if gate is not None:
+            gp = self._rows("gate", gate, (n, T, H, D), (torch.float32,))
+        qn = C.c_void_p(0) if qnorm is None else self._rows("qnorm", qnorm, (D,), (torch.float32,))
+        kn = self._rows("knorm", knorm, (D,), (torch.float32,))
+        ap = C.c_void_p(0) if axis_pos is None else self._rows("axis_pos", axis_pos, (n, T, 3), (torch.int32,))
+        self._ck(self.L.kata_paged_prep(self.h, layer, n, sp, lp, T, ap, None if age0 is None else _i32(age0)[1], qp, kp, vp, _ACT[k.dtype], qn, kn, hp, gp, self._s()))
+        return q16, None, gate
+
+    def decode(self, layer, seq_ids, n_slots, T, q16, gate=None, out=None, out_dtype=torch.float32, accumulate=False):
+        """Attention of the T newest tokens of each sequence over its n_slots slots (kata_paged_decode)."""
+        sa, sp = _i32(seq_ids); la, lp = _i32(n_slots)
+        n = len(sa)
+        if len(la) != n:
+            raise ValueError("one n_slots per sequence")
+        shape = (n, T, self.heads, self.head_dim)
+        out = torch.empty((n, T, self.heads * self.head_dim), dtype=out_dtype, device=q16.device) if out is None else out
+        self._ck(self.L.kata_paged_decode(self.h, layer, n, sp, lp, T, self._rows("q16", q16, shape, (torch.float16,)), C.c_void_p(0) if gate is None else self._rows("gate", gate, shape, (torch.float32,)),
+                                          self._rows("out", out, shape, tuple(_ACT)), _ACT[out.dtype], int(bool(accumulate)), self._s()))
+        return out
+
+    def evict(self, layer, seq_ids, n_slots, keep, seen, sink=0, recent=0, n_layers=1, src=None):
+        """Cuts the sequences to at most ``keep`` slots per KV head by accumulated weight (kata_paged_evict). ``seen``: tokens each sequence has seen (one number, or one per sequence).
+        Returns src [n][kv_heads][keep] ([n_layers] of it for more than one layer): the slot each slot's content came from."""
+        sa, sp = _i32(seq_ids); la, lp = _i32(n_slots)
+        n = len(sa)
+        ea, ep = _i32([seen] * n if isinstance(seen, int) else seen)
+        if len(la) != n or len(ea) != n:
+            raise ValueError("one n_slots (and seen) per sequence")
+        shape = ((n_layers,) if n_layers > 1 else ()) + (n, self.kv_heads, keep)
+        src = torch.empty(shape, dtype=torch.int32, device=torch.device("cuda", self.device)) if src is None else src
+        self._ck(self.L.kata_paged_evict(self.h, layer, n_layers, n, sp, lp, ep, keep, sink, recent, self._rows("src", src, shape, (torch.int32,)), self._s()))
+        return src
+
+    def import_rows(self, layer, seq, slot0, n_rows, src: AttnContext, src_layer, src_seq, src_pos, age0=None):
+        """Copies n_rows rows of a contiguous context into slots slot0.. (kata_paged_import)."""
+        self._ck(self.L.kata_paged_import(self.h, layer, seq, slot0, n_rows, slot0 if age0 is None else age0, src.h, src_layer, src_seq, src_pos, self._s()))

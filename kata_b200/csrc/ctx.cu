@@ -29,6 +29,8 @@ int decode_partial_impl(kata_attn_ctx* h, int32_t layer, int32_t seq, int32_t po
 
 struct kata_attn_ctx { kata::Ctx c; };
 
+namespace kata { Ctx& ctx_of(kata_attn_ctx* h) { return h->c; } }   // for the paged cache, which copies rows out of a contiguous one
+
 using kata::Ctx;
 
 namespace {

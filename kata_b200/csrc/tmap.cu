@@ -2,7 +2,7 @@
 // the library does not link against libcuda.
 #include <cudaTypedefs.h>
 
-#include "kata_internal.cuh"
+#include "paged_internal.cuh"
 
 namespace kata {
 
@@ -37,6 +37,20 @@ bool make_tile_tmap(CUtensorMap* out, void* base, int elt, int64_t rows, int box
     const cuuint32_t box[4] = {inner, (cuuint32_t)box_rows, (cuuint32_t)box_blocks, 1u};
     const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
     return encode(out, elt == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rank-5 view of a paged pool's K or V rows: {x: one 128-byte column block, r: 16 rows, c: column blocks of a head row, g: 16-row groups, h: KV heads}. A box of
+// {block, 16 rows, all blocks, box_groups groups, 1 head} brings one or two 16-slot groups of a head from anywhere in the pool with one TMA
+// instruction and lands as [group][block][16 rows][128 bytes].
+bool make_paged_tmap(CUtensorMap* out, void* base, int elt, int64_t rows, int kv_heads, int head_dim, int box_groups) {
+    PFN_cuTensorMapEncodeTiled encode = get_encode(); if (!encode) return false;
+    const cuuint32_t inner = 128u / (cuuint32_t)elt, blocks = (cuuint32_t)head_dim / inner; const cuuint64_t row = (cuuint64_t)kv_heads * head_dim * elt;
+    const cuuint64_t gdim[5] = {inner, 16, blocks, (cuuint64_t)rows / 16, (cuuint64_t)kv_heads};
+    const cuuint64_t gstride[4] = {row, 128u, row * 16, (cuuint64_t)head_dim * elt};
+    const cuuint32_t box[5] = {inner, 16u, blocks, (cuuint32_t)box_groups, 1u};
+    const cuuint32_t estr[5] = {1u, 1u, 1u, 1u, 1u};
+    return encode(out, elt == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, base, gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
