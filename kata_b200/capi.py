@@ -5,6 +5,7 @@ hand-written CUDA kernels. There is no CPU or PyTorch fallback: if the library i
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import os
 
@@ -61,8 +62,11 @@ def lib() -> C.CDLL:
         L.kata_attn_kv_plane_row_bytes.restype = C.c_size_t
         L.kata_attn_kv_plane_ptr.restype = C.c_void_p
         L.kata_attn_launch_count.restype = C.c_uint64
-        for name in EXPORTS + PAGED_EXPORTS:
+        for name in EXPORTS:
             getattr(L, name)
+        for name, (res, args) in _PAGED_SIGNATURES.items():
+            f = getattr(L, name)
+            f.restype, f.argtypes = res, args
         _lib = L
     return _lib
 
@@ -420,13 +424,25 @@ class PeerExchange:
             self.h = C.c_void_p()
 
 
-PAGED_EXPORTS = [
-    "kata_pages_create", "kata_pages_destroy", "kata_pages_reserve", "kata_pages_trim", "kata_pages_fork", "kata_pages_count", "kata_pages_get", "kata_pages_free_count", "kata_pages_owners",
-    "kata_paged_create", "kata_paged_destroy", "kata_paged_last_error", "kata_paged_launch_count", "kata_paged_check", "kata_paged_plane_ptr", "kata_paged_reserve", "kata_paged_trim", "kata_paged_fork",
-    "kata_paged_table", "kata_paged_prep", "kata_paged_decode", "kata_paged_evict", "kata_paged_import", "kata_paged_decode_plan",
-]
+_P, _I = C.c_void_p, C.c_int32
+_PAGED_SIGNATURES = {   # declared, so that addresses and numbers pass as plain integers
+    "kata_pages_create": (_I, [_I, _I, _I, _I, _P]), "kata_pages_destroy": (_I, [_P]), "kata_pages_reserve": (_I, [_P, _I, _I]), "kata_pages_trim": (_I, [_P, _I, _I]),
+    "kata_pages_fork": (_I, [_P, _I, _I, _I, _P, _P, _P]), "kata_pages_count": (_I, [_P, _I]), "kata_pages_get": (_I, [_P, _I, _P, _I]), "kata_pages_free_count": (_I, [_P]), "kata_pages_owners": (_I, [_P, _I]),
+    "kata_paged_create": (_I, [_P, _P]), "kata_paged_destroy": (_I, [_P]), "kata_paged_last_error": (C.c_char_p, [_P]), "kata_paged_launch_count": (C.c_uint64, [_P]), "kata_paged_check": (_I, [_P, _P]),
+    "kata_paged_plane_ptr": (_P, [_P, _I, _I]), "kata_paged_reserve": (_I, [_P, _I, _I, _P]), "kata_paged_trim": (_I, [_P, _I, _I]), "kata_paged_fork": (_I, [_P, _I, _I, _I, _P]), "kata_paged_table": (_P, [_P]),
+    "kata_paged_prep": (_I, [_P, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P]), "kata_paged_decode": (_I, [_P, _I, _I, _P, _P, _I, _P, _P, _P, _I, _I, _P]),
+    "kata_paged_evict": (_I, [_P, _I, _I, _I, _P, _P, _P, _I, _I, _I, _P, _P]), "kata_paged_import": (_I, [_P, _I, _I, _I, _I, _I, _P, _I, _I, _I, _P]),
+    "kata_paged_decode_plan": (_I, [_I, _P, _I, _I, _I, _P, _I, _P]),
+}
+PAGED_EXPORTS = list(_PAGED_SIGNATURES)
 _PLANES = ("k", "v", "k_scale", "v_scale", "weight", "age")   # KATA_PAGED_* planes
 PAGED_GATED, PAGED_WEIGHTS = 1, 2
+_F16, _F32, _I32 = (torch.float16,), (torch.float32,), (torch.int32,)
+
+
+def _ints(xs):
+    """int32 array of a sequence of integers: its buffer is what the C call reads."""
+    return array.array("i", xs.reshape(-1).tolist() if isinstance(xs, np.ndarray) else xs)
 
 
 class PagedConfig(C.Structure):
@@ -443,9 +459,6 @@ class PagedContext:
         """``sections``: rotary frequencies per axis (time, height, width), all on the first axis by default. ``planes``: the caller's tensors for planes
         ("k", "v", "k_scale", "v_scale", "weight", "age") in the header's layout, [n_layers] of them; the others are allocated, zero-filled."""
         L = self.L = lib()
-        L.kata_paged_last_error.restype = C.c_char_p
-        L.kata_paged_launch_count.restype = C.c_uint64
-        L.kata_paged_plane_ptr.restype = L.kata_paged_table.restype = C.c_void_p
         self.device = torch.cuda.current_device() if device is None else device
         self.n_layers, self.n_seqs, self.n_pages, self.page_size, self.max_slots = n_layers, n_seqs, n_pages, page_size, max_slots
         self.heads, self.kv_heads, self.head_dim, self.kv_mode, self.gated, self.weights = heads, kv_heads, head_dim, kv_mode, gated, weights
@@ -483,7 +496,7 @@ class PagedContext:
             raise KataError(rc, self.L.kata_paged_last_error(self.h).decode())
 
     def _s(self):
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)   # the context's device, whichever is current
+        return torch._C._cuda_getCurrentRawStream(self.device)   # torch.cuda.current_stream(device).cuda_stream without the object; the context's device, whichever is current
 
     def check(self):
         self._ck(self.L.kata_paged_check(self.h, self._s()))
@@ -502,7 +515,7 @@ class PagedContext:
         self._ck(self.L.kata_paged_fork(self.h, src, dst, n_slots, self._s()))
 
     def pages(self, seq: int) -> list:
-        t = C.c_void_p(self.L.kata_paged_table(self.h))
+        t = self.L.kata_paged_table(self.h)
         n = self.L.kata_pages_count(t, seq)
         if n < 0:
             raise KataError(2, f"sequence id {seq}")
@@ -511,7 +524,7 @@ class PagedContext:
         return list(buf)[:n]
 
     def free_pages(self) -> int:
-        return int(self.L.kata_pages_free_count(C.c_void_p(self.L.kata_paged_table(self.h))))
+        return self.L.kata_pages_free_count(self.L.kata_paged_table(self.h))
 
     def plane(self, layer: int, name: str) -> torch.Tensor:
         """A layer's plane as a tensor that aliases it: k, v [pages][page_size][kv_heads][head_dim], scales [pages][page_size][kv_heads], weight and age [pages][kv_heads][page_size]."""
@@ -530,61 +543,62 @@ class PagedContext:
         return torch.as_tensor(_Alias(), device=torch.device("cuda", self.device))
 
     # ---- the operators
-    def _rows(self, what, t, shape, dtypes):
-        """A device tensor of this shape (any grouping of it) and one of these types, contiguous; raises otherwise."""
-        n = 1
-        for x in shape:
-            n *= x
-        if t.dtype not in dtypes or t.numel() != n or not t.is_cuda or t.device.index != self.device or not t.is_contiguous():
-            raise ValueError(f"{what}: a contiguous tensor {list(shape)} of {dtypes} on device {self.device} is needed, not {list(t.shape)} of {t.dtype} on {t.device}")
-        return C.c_void_p(t.data_ptr())
+    def _at(self, what, t, n, kinds):
+        """The address of a contiguous tensor of n elements of one of these types on the context's device; raises otherwise."""
+        if t.dtype not in kinds or t.numel() != n or t.get_device() != self.device or not t.is_contiguous():
+            raise ValueError(f"{what}: a contiguous tensor of {n} elements of {kinds} on device {self.device} is needed, not {list(t.shape)} of {t.dtype} on {t.device}")
+        return t.data_ptr()
 
     def prep(self, layer, seq_ids, slot0, T, q, k, v, qnorm, knorm, axis_pos=None, age0=None, q16=None, gate=None):
         """Norm, rotary positions and append of T tokens per sequence into slots slot0.. (kata_paged_prep). q [n][T][heads][(2) head_dim] or None, k, v [n][T][kv_heads][head_dim], axis_pos int32
         [n][T][3] or None (text: age0 + t on every axis). Returns (q16, None, gate) as AttnContext.prep does."""
-        sa, sp = _i32(seq_ids); la, lp = _i32(slot0)
-        n, H, KH, D = len(sa), self.heads, self.kv_heads, self.head_dim
-        if len(la) != n or (age0 is not None and len(age0) != n):
+        ids, at0, ages, D = _ints(seq_ids), _ints(slot0), None if age0 is None else _ints(age0), self.head_dim
+        n = len(ids)
+        if len(at0) != n or (ages is not None and len(ages) != n):
             raise ValueError("one slot0 (and age0) per sequence")
-        act = (k.dtype,) if k.dtype in _ACT else tuple(_ACT)
-        kp, vp = self._rows("k", k, (n, T, KH, D), act), self._rows("v", v, (n, T, KH, D), act)
-        qp = gp = hp = C.c_void_p(0)
+        act, nq, nk = (k.dtype,) if k.dtype in _ACT else tuple(_ACT), n * T * self.heads * D, n * T * self.kv_heads * D
+        kp, vp = self._at("k", k, nk, act), self._at("v", v, nk, act)
+        qp = gp = hp = None
         if q is not None:
-            qp = self._rows("q", q, (n, T, H, D * (2 if self.gated else 1)), act)
-            q16 = torch.empty((n, T, H * D), dtype=torch.float16, device=k.device) if q16 is None else q16
-            gate = torch.empty((n, T, H * D), dtype=torch.float32, device=k.device) if gate is None and self.gated else gate
-            hp = self._rows("q16", q16, (n, T, H, D), (torch.float16,))
+            qp = self._at("q", q, nq * (2 if self.gated else 1), act)
+            q16 = torch.empty((n, T, self.heads * D), dtype=torch.float16, device=k.device) if q16 is None else q16
+            gate = torch.empty((n, T, self.heads * D), dtype=torch.float32, device=k.device) if gate is None and self.gated else gate
+            hp = self._at("q16", q16, nq, _F16)
         if gate is not None:
-            gp = self._rows("gate", gate, (n, T, H, D), (torch.float32,))
-        qn = C.c_void_p(0) if qnorm is None else self._rows("qnorm", qnorm, (D,), (torch.float32,))
-        kn = self._rows("knorm", knorm, (D,), (torch.float32,))
-        ap = C.c_void_p(0) if axis_pos is None else self._rows("axis_pos", axis_pos, (n, T, 3), (torch.int32,))
-        self._ck(self.L.kata_paged_prep(self.h, layer, n, sp, lp, T, ap, None if age0 is None else _i32(age0)[1], qp, kp, vp, _ACT[k.dtype], qn, kn, hp, gp, self._s()))
+            gp = self._at("gate", gate, nq, _F32)
+        rc = self.L.kata_paged_prep(self.h, layer, n, ids.buffer_info()[0], at0.buffer_info()[0], T, None if axis_pos is None else self._at("axis_pos", axis_pos, n * T * 3, _I32), None if ages is None else ages.buffer_info()[0],
+                                    qp, kp, vp, _ACT[k.dtype], None if qnorm is None else self._at("qnorm", qnorm, D, _F32), self._at("knorm", knorm, D, _F32), hp, gp, self._s())
+        if rc:
+            self._ck(rc)
         return q16, None, gate
 
     def decode(self, layer, seq_ids, n_slots, T, q16, gate=None, out=None, out_dtype=torch.float32, accumulate=False):
         """Attention of the T newest tokens of each sequence over its n_slots slots (kata_paged_decode)."""
-        sa, sp = _i32(seq_ids); la, lp = _i32(n_slots)
-        n = len(sa)
-        if len(la) != n:
+        ids, held = _ints(seq_ids), _ints(n_slots)
+        n = len(ids)
+        if len(held) != n:
             raise ValueError("one n_slots per sequence")
-        shape = (n, T, self.heads, self.head_dim)
+        nq = n * T * self.heads * self.head_dim
+        qp = self._at("q16", q16, nq, _F16)
         out = torch.empty((n, T, self.heads * self.head_dim), dtype=out_dtype, device=q16.device) if out is None else out
-        self._ck(self.L.kata_paged_decode(self.h, layer, n, sp, lp, T, self._rows("q16", q16, shape, (torch.float16,)), C.c_void_p(0) if gate is None else self._rows("gate", gate, shape, (torch.float32,)),
-                                          self._rows("out", out, shape, tuple(_ACT)), _ACT[out.dtype], int(bool(accumulate)), self._s()))
+        rc = self.L.kata_paged_decode(self.h, layer, n, ids.buffer_info()[0], held.buffer_info()[0], T, qp, None if gate is None else self._at("gate", gate, nq, _F32), self._at("out", out, nq, _ACT), _ACT[out.dtype], 1 if accumulate else 0, self._s())
+        if rc:
+            self._ck(rc)
         return out
 
     def evict(self, layer, seq_ids, n_slots, keep, seen, sink=0, recent=0, n_layers=1, src=None):
         """Cuts the sequences to at most ``keep`` slots per KV head by accumulated weight (kata_paged_evict). ``seen``: tokens each sequence has seen (one number, or one per sequence).
         Returns src [n][kv_heads][keep] ([n_layers] of it for more than one layer): the slot each slot's content came from."""
-        sa, sp = _i32(seq_ids); la, lp = _i32(n_slots)
-        n = len(sa)
-        ea, ep = _i32([seen] * n if isinstance(seen, int) else seen)
-        if len(la) != n or len(ea) != n:
+        ids, held = _ints(seq_ids), _ints(n_slots)
+        n = len(ids)
+        total = _ints([seen] * n if isinstance(seen, int) else seen)
+        if len(held) != n or len(total) != n:
             raise ValueError("one n_slots (and seen) per sequence")
-        shape = ((n_layers,) if n_layers > 1 else ()) + (n, self.kv_heads, keep)
+        shape = (n, self.kv_heads, keep) if n_layers == 1 else (n_layers, n, self.kv_heads, keep)
         src = torch.empty(shape, dtype=torch.int32, device=torch.device("cuda", self.device)) if src is None else src
-        self._ck(self.L.kata_paged_evict(self.h, layer, n_layers, n, sp, lp, ep, keep, sink, recent, self._rows("src", src, shape, (torch.int32,)), self._s()))
+        rc = self.L.kata_paged_evict(self.h, layer, n_layers, n, ids.buffer_info()[0], held.buffer_info()[0], total.buffer_info()[0], keep, sink, recent, self._at("src", src, n_layers * n * self.kv_heads * keep, _I32), self._s())
+        if rc:
+            self._ck(rc)
         return src
 
     def import_rows(self, layer, seq, slot0, n_rows, src: AttnContext, src_layer, src_seq, src_pos, age0=None):

@@ -5,20 +5,27 @@
 // Bound by HBM (4096 bytes of K+V per slot at fp16 with 4 heads of 256, each read once), so the work split is that of the contiguous decode kernel:
 // the tiles (16 or 32 slots of one KV head, 16 KiB of K+V) of all (sequence, KV head) segments form one list, cut into one contiguous range per SM, the
 // ranges' partial rows joined by the last CTA of a segment (at most 8 of them) or by a combine grid. Inside a CTA four rings of a score warp and two value warps take
-// the tiles in turn; a producer warp refills the rings' stages with TMA. What pages change:
+// the tiles in turn; producer warps refill the
+// rings' stages with TMA. What pages change:
 //  - A tile is made of 16-slot groups, and a group never crosses a page (pages are powers of two from 16 slots on). The tensor map is a rank-5 view of
 //    the pool, {128-byte column block, 16 rows, column blocks, 16-row groups, KV heads}: the group is a coordinate, so one instruction
 //    brings the 16 or 32 slots of a tile wherever their page lies, in the same shared-memory order ([group][column block][16 rows][128 bytes], swizzled) for
 //    every page size. Pages of 16 slots under 32-slot tiles take two instructions.
-//  - The producer reads the page number of a tile three tiles before it needs it, the score warp that of its int8 scales six tiles before: neither waits for a table look-up.
+//  - The producer reads the page number of a tile three tiles before it needs it. In the int8 mode a ring has a producer warp
+//    of its own, whose lanes fetch the slots' K and V scales as well, three tiles ahead, and leave them in shared memory: with the loads in the score warp it waited for them (359 us for 32 sequences of 300 to
+//    32K slots), and so it did with one warp for the four rings' scales (352 us).
 //  - Groups behind the last slot repeat the last page (their table entry may not exist); such slots are masked, and their V rows zeroed in shared
 //    memory, so whatever lies there (NaN included) has no part in the result.
 // Head layouts: head_dim 256 or 128, up to 16 query heads per KV head; tokens beyond 16 / group run as further passes.
 //
+// The matrix instructions take the keys (and the head dims of V) as their 16 rows and the query rows as their 8 columns: S^T = K Q^T, O^T = V^T P^T. One token of up to 8 heads
+// per KV head then costs half the instructions, softmax and registers of a 16-row block (NR = 1 against NR = 2 column tiles); the query's fragments stay in registers
+// for the whole segment. With the query rows as the 16 rows instead, 32 sequences of 300 to 32K int8 slots took 280 us.
+//
 // Precision: fp16 products, fp32 sums. The exponent carries an offset (kPShift) so that p lies high in fp16's range: it cancels in p / l and keeps
-// small p out of the subnormals. p is rounded to fp16 before P.V as in the contiguous kernel (relative error 2^-11 at most, what the bf16 or fp16
-// output is rounded by anyway); FINE (fp32 outputs) carries it in two fp16 terms and takes int8 codes without the 1152 bias whose subtraction would cost
-// some ten bits.
+// small p out of the subnormals. p goes into P.V in two fp16 terms (about 22 bits; int8 caches with 16-bit outputs: one term, 2^-11 relative, there the second costs time), int8 codes are taken
+// without the 1152 bias of the contiguous kernel (whose subtraction costs some ten bits), and a tile's P.V is formed in fresh accumulators and added to O with a rounded fma (the matrix
+// unit truncates its sums: over hundreds of tiles that showed as 3e-6 in fp32 outputs).
 #include <algorithm>
 
 #include "attn_tile.cuh"
@@ -29,26 +36,28 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kRings = 4, kWarps = 3 * kRings + 1, kThreads = kWarps * 32, kMaxStages = 8;
+constexpr int kRings = 4, kMaxStages = 6;
 
-template <int HD, bool K8, bool FINE> struct PGeo {
+// The barrier block: per ring and stage 'full' and 'empty', then per ring two 'P full' and two 'P empty'.
+constexpr int kOffEBars = kRings * kMaxStages * 8, kOffPBars = 2 * kOffEBars, kBarBytes = kOffPBars + kRings * 32;
+
+template <int HD, bool K8> struct PGeo {
+    static constexpr int kThreads = (3 * kRings + (K8 ? kRings : 1)) * 32;               // fp16: one producer warp, lane r for ring r (in step: 142 us for eight sequences of 16K to 32K slots, 154 with one per ring); int8: one per ring
     static constexpr int kRowBytes = HD * (K8 ? 1 : 2), kNB = kRowBytes / 128;           // bytes and 128-byte column blocks of a head row
     static constexpr int kNK = (HD == 256 && !K8) ? 1 : 2, kTile = 16 * kNK;             // 16-slot groups and slots per tile
     static constexpr int kGroupBytes = 16 * kRowBytes, kHalfBytes = kNK * kGroupBytes;   // K (or V) of one group, of one tile
     static constexpr int kStageBytes = 2 * kHalfBytes, kStages = kStageBytes == 16384 ? 3 : 6;
     static constexpr int kMergeStride = HD + 8;                                          // floats per row of the cross-ring merge buffer
     static constexpr int kRingBytes = kStages * kStageBytes;
-    static constexpr int kQStride = HD * 2 + 16;
-    static constexpr int kPStride = 32 * kNK + 16, kPTerm = 16 * kPStride, kPBytes = kPTerm * (FINE ? 2 : 1) + 64;   // a P slot: one or two fp16 blocks, 16 rescale factors
+    static constexpr int kQStride = HD * 2 + 16, kQBytes = 16 * kQStride;                // the query block: fp16 rows, 16 bytes of padding
+    static constexpr int kPStride = 32 * kNK + 16, kPTerm = 16 * kPStride, kPBytes = 2 * kPTerm + 64;   // a P slot: two fp16 blocks (heads and remainders), 16 rescale factors
     static constexpr int kPShift = K8 ? 5 : 15;                                          // p is carried as 2^kPShift * p (int8: p times a scale up to 516 has to stay below 65504)
-    static constexpr int kOffBars = 16 * kQStride, kOffQsum = kOffBars + 704, kOffMl = kOffQsum + 64, kOffPair = kOffMl + 512, kOffStages = kOffPair + kRings * 2 * kPBytes;
+    static constexpr int kOffBars = kQBytes, kOffMl = kOffBars + kBarBytes, kOffPair = kOffMl + 512, kOffScale = kOffPair + kRings * 2 * kPBytes, kOffStages = kOffScale + (K8 ? kRings * kStages * 128 : 0);   // scales: [ring][stage][32 slots] K and V packed
     static constexpr int kSmem = kOffStages + 1024 + kRings * kRingBytes;
     static_assert(16 * kMergeStride * 4 <= kRingBytes && kSmem <= 232448, "shared memory");
 };
-constexpr int kOffEBars = kRings * kMaxStages * 8, kOffPBars = 2 * kOffEBars;   // inside the barrier block: 'full', 'empty', then per ring two 'P full' and two 'P empty'
-static_assert(kOffPBars + kRings * 32 <= 704, "barrier block");
-
 struct PagedPlan {
+    int32_t two_terms;                                              // P in two fp16 terms (fp32 outputs; always where it is free)
     int32_t n, T, group, kv_heads, n_ctas, q_tiles, r_tiles, cps;   // as in the contiguous kernel: CTA c owns tiles [c*q + min(c,r), ..), or (cps > 0) a share of one segment
     int32_t tok_stride, tok0, page_shift, width, groups_per_box, merge_in_kernel;
     int64_t layer_row0;
@@ -74,157 +83,185 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* tmap, int 
                  ::"r"(dst), "l"(tmap), "r"(x), "r"(r), "r"(c), "r"(g), "r"(h), "r"(bar) : "memory");
 }
 
-// Score warp, one tile: s[nt][e] = q_row . k of n-tile nt (8 slots: key0 + 8*nt + 2*t4 + e; elements 2, 3: row g + 8), scaled (int8) and masked.
-template <int HD, bool K8, bool FINE>
-__device__ __forceinline__ void paged_scores(const uint32_t q_sm, const uint32_t k_sm, const int key0, const int lim0, const int lim1, const float (&ks)[2 * PGeo<HD, K8, FINE>::kNK][2], const float (&qs)[2],
-                                             const int lane, float (&s)[2 * PGeo<HD, K8, FINE>::kNK][4]) {
-    using G = PGeo<HD, K8, FINE>; constexpr int NK = G::kNK, NT = 2 * NK;
-    const int t4 = lane & 3; const uint32_t rx = lane & 7, q1 = (lane >> 3) & 1;
-    const uint32_t qa = q_sm + (lane & 15) * G::kQStride + (lane >> 4) * 16, ka = k_sm + (rx + ((lane >> 4) << 3)) * 128;
-    const uint32_t ko[4] = {((0 + q1) ^ rx) << 4, ((2 + q1) ^ rx) << 4, ((4 + q1) ^ rx) << 4, ((6 + q1) ^ rx) << 4};
-    float s2[NT][4];   // a second accumulator chain per n-tile
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) { s[nt][e] = 0.0f; s2[nt][e] = 0.0f; }
-    if (!K8) {
-#pragma unroll
-        for (int kk = 0; kk < HD / 16; kk += 2) {
-            uint32_t a0, a1, a2, a3, c0, c1, c2, c3;
-            ldsm_x4(qa + kk * 32, a0, a1, a2, a3); ldsm_x4(qa + kk * 32 + 32, c0, c1, c2, c3);
-#pragma unroll
-            for (int sb = 0; sb < NK; sb++) {
-                uint32_t b0, b1, b2, b3, d0, d1, d2, d3; const uint32_t kb = ka + sb * G::kGroupBytes + (kk >> 2) * 2048;
-                ldsm_x4(kb + ko[kk & 3], b0, b1, b2, b3); ldsm_x4(kb + ko[(kk & 3) + 1], d0, d1, d2, d3);
-                mma16816(s[2 * sb], a0, a1, a2, a3, b0, b1); mma16816(s[2 * sb + 1], a0, a1, a2, a3, b2, b3);
-                mma16816(s2[2 * sb], c0, c1, c2, c3, d0, d1); mma16816(s2[2 * sb + 1], c0, c1, c2, c3, d2, d3);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int k2 = 0; k2 < HD / 32; k2++) {   // a 16-byte chunk is a 16-dim block
-            uint32_t a0, a1, a2, a3, c0, c1, c2, c3;
-            ldsm_x4(qa + (2 * k2) * 32, a0, a1, a2, a3); ldsm_x4(qa + (2 * k2 + 1) * 32, c0, c1, c2, c3);
-#pragma unroll
-            for (int sb = 0; sb < NK; sb++) {
-                uint32_t r0, r1, r2, r3;
-                ldsm_x4(ka + sb * G::kGroupBytes + (k2 >> 2) * 2048 + ko[k2 & 3], r0, r1, r2, r3);
-                r0 ^= 0x80808080u; r1 ^= 0x80808080u; r2 ^= 0x80808080u; r3 ^= 0x80808080u;
-                auto dq = [](uint32_t x, uint32_t sel) { return FINE ? deq2(x, sel) : deq2_biased(x, sel); };
-                mma16816(s[2 * sb], a0, a1, a2, a3, dq(r0, 0x4140u), dq(r0, 0x4342u)); mma16816(s[2 * sb + 1], a0, a1, a2, a3, dq(r2, 0x4140u), dq(r2, 0x4342u));
-                mma16816(s2[2 * sb], c0, c1, c2, c3, dq(r1, 0x4140u), dq(r1, 0x4342u)); mma16816(s2[2 * sb + 1], c0, c1, c2, c3, dq(r3, 0x4140u), dq(r3, 0x4342u));
-            }
-        }
-    }
-    const float b0 = (K8 && !FINE) ? kI8Bias * qs[0] : 0.0f, b1 = (K8 && !FINE) ? kI8Bias * qs[1] : 0.0f;   // biased codes: the scores were formed against code + 1152
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            float x = s[nt][e] + s2[nt][e], y = s[nt][2 + e] + s2[nt][2 + e];
-            if (K8) { x = (x - b0) * ks[nt][e]; y = (y - b1) * ks[nt][e]; }
-            const int key = key0 + nt * 8 + 2 * t4 + e;   // masked by select: what lies there may be anything
-            s[nt][e] = key < lim0 ? x : -INFINITY; s[nt][2 + e] = key < lim1 ? y : -INFINITY;
-        }
+__device__ __forceinline__ void stsm_x4_t(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
+}
+__device__ __forceinline__ void stsm_x2_t(uint32_t addr, uint32_t r0, uint32_t r1) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1,%2};" ::"r"(addr), "r"(r0), "r"(r1) : "memory");
 }
 
-// Online softmax of a tile's scores: pr = 2^shift * exp(s - m), the state and the rescale factors of rows g and g + 8 brought up to date.
-template <int NT, int SHIFT>
-__device__ __forceinline__ void paged_softmax(const float (&s)[NT][4], ScoreState& st, float (&pr)[NT][4], float& al0, float& al1) {
-    float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) { mx0 = fmaxf(mx0, fmaxf(s[nt][0], s[nt][1])); mx1 = fmaxf(mx1, fmaxf(s[nt][2], s[nt][3])); }
-    mx0 *= kLog2e; mx1 *= kLog2e;
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1)); mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1)); mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-    const float mn0 = fmaxf(st.m0, mx0), mn1 = fmaxf(st.m1, mx1);
-    al0 = (mn0 == -INFINITY) ? 1.0f : ex2(st.m0 - mn0); al1 = (mn1 == -INFINITY) ? 1.0f : ex2(st.m1 - mn1);
-    const float sub0 = (mn0 == -INFINITY) ? 0.0f : mn0 - SHIFT, sub1 = (mn1 == -INFINITY) ? 0.0f : mn1 - SHIFT;
-    st.m0 = mn0; st.m1 = mn1;
-    float sum0 = 0.0f, sum1 = 0.0f;
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        pr[nt][0] = ex2(fmaf(s[nt][0], kLog2e, -sub0)); pr[nt][1] = ex2(fmaf(s[nt][1], kLog2e, -sub0));
-        pr[nt][2] = ex2(fmaf(s[nt][2], kLog2e, -sub1)); pr[nt][3] = ex2(fmaf(s[nt][3], kLog2e, -sub1));
-        sum0 += pr[nt][0] + pr[nt][1]; sum1 += pr[nt][2] + pr[nt][3];
-    }
-    st.l0 = st.l0 * al0 + sum0; st.l1 = st.l1 * al1 + sum1;
+// Fragments (m16n8k16, g = lane / 4, t4 = lane % 4). S^T: elements 0, 1 = slot g, query rows 2 * t4 and the next; elements 2, 3 = slot g + 8. O^T: the same with head dims for slots.
+// int8 codes lie four dims (K) or two dims of two slots (V) to a register: their dims are taken in the order 4*t4 + {0, 1}, 4*t4 + {2, 3} (K: the staged
+// query columns are permuted alike) and 2*g, 2*g + 1 (V).
+
+// The query's fragments of k-steps kk, kk + 1 for column tile nr
+__device__ __forceinline__ void q_frags(const uint32_t q_sm, const int stride, const int nr, const int kk, const int lane, uint32_t (&f0)[2], uint32_t (&f1)[2]) {
+    ldsm_x4(q_sm + (nr * 8 + (lane & 7)) * stride + (2 * kk + (lane >> 3)) * 16, f0[0], f0[1], f1[0], f1[1]);
 }
 
-template <int HD, bool K8, bool FINE>
-__device__ __forceinline__ void paged_publish(const uint32_t p_sm, float* alpha, const float (&pr)[2 * PGeo<HD, K8, FINE>::kNK][4], const float al0, const float al1, const int lane) {
-    using G = PGeo<HD, K8, FINE>; const int g = lane >> 2, t4 = lane & 3;
+// Score warp, one tile: s[sb][nr] = the fragment of 16-slot group sb and column tile nr, scaled (int8). qf: the query's fragments (NR = 1).
+template <int HD, bool K8, int NR>
+__device__ __forceinline__ void paged_scores(const uint32_t q_sm, const uint32_t k_sm, const uint32_t (&qf)[HD / 16][2], const float (&ks)[PGeo<HD, K8>::kNK][2], const int lane, float (&s)[PGeo<HD, K8>::kNK][NR][4]) {
+    using G = PGeo<HD, K8>; constexpr int NK = G::kNK;
+    const uint32_t rx = lane & 7, hi = lane >> 4, ka = k_sm + (rx + ((lane >> 3) & 1) * 8) * 128;   // lanes 0-15: slots 0-15 at one chunk, lanes 16-31: at the next
+    const uint32_t ko[4] = {((0 + hi) ^ rx) << 4, ((2 + hi) ^ rx) << 4, ((4 + hi) ^ rx) << 4, ((6 + hi) ^ rx) << 4};
+    float s2[NK][NR][4];   // a second accumulator chain
 #pragma unroll
-    for (int nt = 0; nt < 2 * G::kNK; nt++)
+    for (int sb = 0; sb < NK; sb++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const float x = pr[nt][2 * h], y = pr[nt][2 * h + 1]; const uint32_t at = p_sm + (g + 8 * h) * G::kPStride + (8 * nt + 2 * t4) * 2, hi = pack_h2(x, y);
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(hi) : "memory");
-            if (FINE) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + G::kPTerm), "r"(pack_h2(x - f.x, y - f.y)) : "memory");
-            }
+        for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) { s[sb][nr][e] = 0.0f; s2[sb][nr][e] = 0.0f; }
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; kk += 2) {   // two k-steps of 16 dims
+        uint32_t b[2][NR][2];
+        if (NR == 1) { b[0][0][0] = qf[kk][0]; b[0][0][1] = qf[kk][1]; b[1][0][0] = qf[kk + 1][0]; b[1][0][1] = qf[kk + 1][1]; }
+        else {
+#pragma unroll
+            for (int nr = 0; nr < NR; nr++) q_frags(q_sm, G::kQStride, nr, kk, lane, b[0][nr], b[1][nr]);
         }
-    if (t4 == 0) { alpha[g] = al0; alpha[g + 8] = al1; }
-}
-
-// Value warp, one tile: O = O * alpha + P V on half vh of the head dims.
-template <int HD, bool K8, bool FINE>
-__device__ __forceinline__ void paged_values(const uint32_t v_sm, const uint32_t p_sm, const float* alpha, ValueStateT<HD / 16>& st, const int lane, const int vh) {
-    using G = PGeo<HD, K8, FINE>; constexpr int NK = G::kNK, NJ = HD / 16;
-    const int g = lane >> 2; const float al0 = alpha[g], al1 = alpha[g + 8];
-    uint32_t pa[NK][4], pl[NK][4];
-#pragma unroll
-    for (int sb = 0; sb < NK; sb++) {
-        const uint32_t at = p_sm + (lane & 15) * G::kPStride + sb * 32 + (lane >> 4) * 16;
-        ldsm_x4(at, pa[sb][0], pa[sb][1], pa[sb][2], pa[sb][3]);
-        if (FINE) ldsm_x4(at + G::kPTerm, pl[sb][0], pl[sb][1], pl[sb][2], pl[sb][3]);
-    }
-    if (__any_sync(0xffffffffu, al0 != 1.0f || al1 != 1.0f)) {
-#pragma unroll
-        for (int j = 0; j < NJ; j++) { st.o[j][0] *= al0; st.o[j][1] *= al0; st.o[j][2] *= al1; st.o[j][3] *= al1; }
-    }
-    if (K8 && !FINE) {   // sums of the rounded P: the bias term of the biased codes
-        float a0 = 0.0f, a1 = 0.0f;
 #pragma unroll
         for (int sb = 0; sb < NK; sb++) {
-            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&pa[sb][0])), f1 = __half22float2(*reinterpret_cast<const __half2*>(&pa[sb][1]));
-            const float2 f2 = __half22float2(*reinterpret_cast<const __half2*>(&pa[sb][2])), f3 = __half22float2(*reinterpret_cast<const __half2*>(&pa[sb][3]));
-            a0 += (f0.x + f0.y) + (f2.x + f2.y); a1 += (f1.x + f1.y) + (f3.x + f3.y);
+            const uint32_t kb = ka + sb * G::kGroupBytes;
+            uint32_t a[2][4];
+            if (!K8) {   // a k-step is two 16-byte chunks
+                ldsm_x4(kb + (kk >> 2) * 2048 + ko[kk & 3], a[0][0], a[0][1], a[0][2], a[0][3]); ldsm_x4(kb + (kk >> 2) * 2048 + ko[(kk & 3) + 1], a[1][0], a[1][1], a[1][2], a[1][3]);
+            } else {     // a k-step is one chunk of 16 codes
+                uint32_t r[4]; ldsm_x4(kb + (kk >> 3) * 2048 + ko[(kk >> 1) & 3], r[0], r[1], r[2], r[3]);
+#pragma unroll
+                for (int x = 0; x < 4; x++) { r[x] ^= 0x80808080u; a[x >> 1][x & 1] = deq2(r[x], 0x4140u); a[x >> 1][2 + (x & 1)] = deq2(r[x], 0x4342u); }
+            }
+#pragma unroll
+            for (int nr = 0; nr < NR; nr++) { mma16816(s[sb][nr], a[0][0], a[0][1], a[0][2], a[0][3], b[0][nr][0], b[0][nr][1]); mma16816(s2[sb][nr], a[1][0], a[1][1], a[1][2], a[1][3], b[1][nr][0], b[1][nr][1]); }
         }
-        st.ps0 = st.ps0 * al0 + a0; st.ps1 = st.ps1 * al1 + a1;
     }
-    const uint32_t rx = lane & 7, ud = lane >> 4;
-    constexpr int kC0 = HD * (K8 ? 1 : 2) / 2 / 16;   // first 16-byte chunk of the second half of a head row
-    const uint32_t va = v_sm + (rx + ((lane >> 3) & 1) * 8) * 128 + (uint32_t)(vh * (kC0 >> 3)) * 2048, cb = (uint32_t)vh * (kC0 & 7);   // 128-wide int8 heads: the halves share a column block
-    const uint32_t vo[4] = {((cb + 0 + ud) ^ rx) << 4, ((cb + 2 + ud) ^ rx) << 4, ((cb + 4 + ud) ^ rx) << 4, ((cb + 6 + ud) ^ rx) << 4};
-    auto mma = [&](float (&c)[4], int sb, uint32_t b0, uint32_t b1) {
-        mma16816(c, pa[sb][0], pa[sb][1], pa[sb][2], pa[sb][3], b0, b1);
-        if (FINE) mma16816(c, pl[sb][0], pl[sb][1], pl[sb][2], pl[sb][3], b0, b1);
-    };
-    if (!K8) {
 #pragma unroll
-        for (int j2 = 0; j2 < NJ / 2; j2++)
+    for (int sb = 0; sb < NK; sb++)
+#pragma unroll
+        for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) { s[sb][nr][e] += s2[sb][nr][e]; if (K8) s[sb][nr][e] *= ks[sb][e >> 1]; }
+}
+
+// Online softmax state of query rows nr * 8 + 2 * t4 + {0, 1}: maximum (log2 units) and this lane's share of the sum
+template <int NR> struct RowsState { float m[NR][2], l[NR][2]; };
+
+// pr = 2^SHIFT * exp(s - m) in place of s; the state and the rescale factors brought up to date.
+template <int NK, int NR, int SHIFT>
+__device__ __forceinline__ void paged_softmax(float (&s)[NK][NR][4], RowsState<NR>& st, float (&al)[NR][2]) {
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int sb = 0; sb < NK; sb++) mx = fmaxf(mx, fmaxf(s[sb][nr][e], s[sb][nr][2 + e]));
+            mx *= kLog2e;
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float mn = fmaxf(st.m[nr][e], mx), sub = (mn == -INFINITY) ? 0.0f : mn - SHIFT;
+            al[nr][e] = (mn == -INFINITY) ? 1.0f : ex2(st.m[nr][e] - mn); st.m[nr][e] = mn;
+            float sum = 0.0f;
 #pragma unroll
             for (int sb = 0; sb < NK; sb++) {
-                uint32_t b0, b1, b2, b3; ldsm_x4_t(va + sb * G::kGroupBytes + (j2 >> 2) * 2048 + vo[j2 & 3], b0, b1, b2, b3);
-                mma(st.o[2 * j2], sb, b0, b1); mma(st.o[2 * j2 + 1], sb, b2, b3);
+                s[sb][nr][e] = ex2(fmaf(s[sb][nr][e], kLog2e, -sub)); s[sb][nr][2 + e] = ex2(fmaf(s[sb][nr][2 + e], kLog2e, -sub));
+                sum += s[sb][nr][e] + s[sb][nr][2 + e];
             }
-    } else {
+            st.l[nr][e] = st.l[nr][e] * al[nr][e] + sum;
+        }
+}
+
+// P goes to shared memory as [query row][slot] fp16, heads and (two terms) remainders; the rescale factors behind it.
+template <int HD, bool K8, int NR>
+__device__ __forceinline__ void paged_publish(const uint32_t p_sm, float* alpha, const float (&pr)[PGeo<HD, K8>::kNK][NR][4], const float (&al)[NR][2], const int two_terms, const int lane) {
+    using G = PGeo<HD, K8>; constexpr int NK = G::kNK;
 #pragma unroll
-        for (int j2 = 0; j2 < NJ / 4; j2++)
+    for (int nr = 0; nr < NR; nr++) {
+        uint32_t hi[2 * NK], lo[2 * NK];   // 8-slot blocks
 #pragma unroll
-            for (int sb = 0; sb < NK; sb++) {
-                uint32_t r0, r1, r2, r3; ldsm_x4_t(va + sb * G::kGroupBytes + vo[j2], r0, r1, r2, r3);
-                r0 ^= 0x80808080u; r1 ^= 0x80808080u; r2 ^= 0x80808080u; r3 ^= 0x80808080u;
-                auto dq = [](uint32_t x, uint32_t sel) { return FINE ? deq2(x, sel) : deq2_biased(x, sel); };
-                mma(st.o[4 * j2 + 0], sb, dq(r0, 0x4240u), dq(r1, 0x4240u)); mma(st.o[4 * j2 + 1], sb, dq(r0, 0x4341u), dq(r1, 0x4341u));
-                mma(st.o[4 * j2 + 2], sb, dq(r2, 0x4240u), dq(r3, 0x4240u)); mma(st.o[4 * j2 + 3], sb, dq(r2, 0x4341u), dq(r3, 0x4341u));
-            }
+        for (int x = 0; x < 2 * NK; x++) {
+            const float u = pr[x >> 1][nr][2 * (x & 1)], v = pr[x >> 1][nr][2 * (x & 1) + 1];
+            hi[x] = pack_h2(u, v);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[x]));
+            lo[x] = pack_h2(u - f.x, v - f.y);
+        }
+        const uint32_t at = p_sm + (nr * 8 + (lane & 7)) * G::kPStride + ((lane >> 3) & (2 * NK - 1)) * 16;
+        if constexpr (NK == 2) { stsm_x4_t(at, hi[0], hi[1], hi[2], hi[3]); if (two_terms) stsm_x4_t(at + G::kPTerm, lo[0], lo[1], lo[2], lo[3]); }
+        else { stsm_x2_t(at, hi[0], hi[1]); if (two_terms) stsm_x2_t(at + G::kPTerm, lo[0], lo[1]); }
+        if (lane < 4) *reinterpret_cast<float2*>(alpha + nr * 8 + 2 * lane) = make_float2(al[nr][0], al[nr][1]);
     }
 }
 
-struct PagedOut { const float* gate; void* out; int32_t kind; float* fin_ml; };   // fin_ml: joined (m, l) per (segment, row), with weights only
+// Value warp, one tile: O^T = O^T * alpha + V^T P^T on half vh of the head dims (HD / 32 tiles of 16 dims).
+template <int HD, int NR> struct ValueAcc {
+    float o[HD / 32][NR][4];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+            for (int nr = 0; nr < NR; nr++) { o[j][nr][0] = o[j][nr][1] = o[j][nr][2] = o[j][nr][3] = 0.0f; }
+    }
+};
+template <int HD, bool K8, int NR, bool TWO>
+__device__ __forceinline__ void paged_values(const uint32_t v_sm, const uint32_t p_sm, const float* alpha, ValueAcc<HD, NR>& st, const int lane, const int vh) {
+    using G = PGeo<HD, K8>; constexpr int NK = G::kNK;
+    float2 al[NR]; uint32_t ph[NR][2 * NK], pl[NR][2 * NK];
+#pragma unroll
+    for (int nr = 0; nr < NR; nr++) {
+        al[nr] = *reinterpret_cast<const float2*>(alpha + nr * 8 + 2 * (lane & 3));
+        const uint32_t at = p_sm + (nr * 8 + (lane & 7)) * G::kPStride + ((lane >> 3) & (2 * NK - 1)) * 16;
+        auto load = [&](uint32_t a, uint32_t (&x)[2 * NK]) {
+            if constexpr (NK == 2) ldsm_x4(a, x[0], x[1], x[2], x[3]);
+            else asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(a));
+        };
+        load(at, ph[nr]);
+        if (TWO) load(at + G::kPTerm, pl[nr]);
+    }
+    const uint32_t rx = lane & 7, q1 = (lane >> 3) & 1, q2 = lane >> 4;
+    constexpr int kC0 = HD * (K8 ? 1 : 2) / 2 / 16;   // first 16-byte chunk of the second half of a head row
+    const uint32_t cb = (uint32_t)vh * (kC0 & 7);     // 128-wide int8 heads: the halves share a column block
+    auto step = [&](int j, int sb, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, float (&c)[NR][4]) {
+#pragma unroll
+        for (int nr = 0; nr < NR; nr++) { mma16816(c[nr], a0, a1, a2, a3, ph[nr][2 * sb], ph[nr][2 * sb + 1]); if (TWO) mma16816(c[nr], a0, a1, a2, a3, pl[nr][2 * sb], pl[nr][2 * sb + 1]); }
+    };
+    auto add = [&](int j, const float (&c)[NR][4]) {
+#pragma unroll
+        for (int nr = 0; nr < NR; nr++) {
+            st.o[j][nr][0] = fmaf(st.o[j][nr][0], al[nr].x, c[nr][0]); st.o[j][nr][1] = fmaf(st.o[j][nr][1], al[nr].y, c[nr][1]);
+            st.o[j][nr][2] = fmaf(st.o[j][nr][2], al[nr].x, c[nr][2]); st.o[j][nr][3] = fmaf(st.o[j][nr][3], al[nr].y, c[nr][3]);
+        }
+    };
+    if (!K8) {   // a tile of 16 dims is two chunks: lanes 0-7 slots 0-7 at the first, 8-15 at the second, 16-31 slots 8-15
+        const uint32_t va = v_sm + (rx + q2 * 8) * 128 + (uint32_t)(vh * (kC0 >> 3)) * 2048;
+        const uint32_t vo[4] = {((0 + q1) ^ rx) << 4, ((2 + q1) ^ rx) << 4, ((4 + q1) ^ rx) << 4, ((6 + q1) ^ rx) << 4};
+#pragma unroll
+        for (int j = 0; j < HD / 32; j++) {
+            float c[NR][4] = {};
+#pragma unroll
+            for (int sb = 0; sb < NK; sb++) {
+                uint32_t a0, a1, a2, a3; ldsm_x4_t(va + sb * G::kGroupBytes + (j >> 2) * 2048 + vo[j & 3], a0, a1, a2, a3);
+                step(j, sb, a0, a1, a2, a3, c);
+            }
+            add(j, c);
+        }
+    } else {     // a tile of 16 dims is one chunk: lanes 0-15 slots 0-15 at one chunk, lanes 16-31 at the next
+        const uint32_t va = v_sm + (rx + q1 * 8) * 128 + (uint32_t)(vh * (kC0 >> 3)) * 2048;
+        const uint32_t vo[4] = {((cb + 0 + q2) ^ rx) << 4, ((cb + 2 + q2) ^ rx) << 4, ((cb + 4 + q2) ^ rx) << 4, ((cb + 6 + q2) ^ rx) << 4};
+#pragma unroll
+        for (int j = 0; j < HD / 32; j += 2) {
+            float c0[NR][4] = {}, c1[NR][4] = {};
+#pragma unroll
+            for (int sb = 0; sb < NK; sb++) {
+                uint32_t r0, r1, r2, r3; ldsm_x4_t(va + sb * G::kGroupBytes + vo[j >> 1], r0, r1, r2, r3);   // r0, r1: slots 0-7, 8-15 of one chunk; r2, r3: of the next
+                r0 ^= 0x80808080u; r1 ^= 0x80808080u; r2 ^= 0x80808080u; r3 ^= 0x80808080u;
+                step(j, sb, deq2(r0, 0x4240u), deq2(r0, 0x4341u), deq2(r1, 0x4240u), deq2(r1, 0x4341u), c0);
+                step(j + 1, sb, deq2(r2, 0x4240u), deq2(r2, 0x4341u), deq2(r3, 0x4240u), deq2(r3, 0x4341u), c1);
+            }
+            add(j, c0); add(j + 1, c1);
+        }
+    }
+}
+
+struct PagedOut { const float* gate; void* out; int32_t kind; float* fin_ml; };   // fin_ml: joined (m, 1 / l) per (segment, row), with weights only
 
 // Final value of row r of a segment, dims d and d + 1: normalised, gated, stored. A row that saw no slot has l = 0 and gets zeros.
 template <int HD> __device__ __forceinline__ void paged_emit(const PagedPlan& p, const PagedOut& o, int b, int kvh, int r, int d, float M, float L, float A0, float A1) {
@@ -234,17 +271,18 @@ template <int HD> __device__ __forceinline__ void paged_emit(const PagedPlan& p,
     if (o.gate) { const float2 gt = *reinterpret_cast<const float2*>(o.gate + oi); y0 *= sigmoid_fast(gt.x); y1 *= sigmoid_fast(gt.y); }
     if (L == 0.0f) { y0 = 0.0f; y1 = 0.0f; }
     store_act2(o.out, oi, y0, y1, o.kind);
-    if (o.fin_ml && d == 0) *reinterpret_cast<float2*>(o.fin_ml + ((int64_t)(b * p.kv_heads + kvh) * 16 + r) * 2) = make_float2(M, L);
+    if (o.fin_ml && d == 0) *reinterpret_cast<float2*>(o.fin_ml + ((int64_t)(b * p.kv_heads + kvh) * 16 + r) * 2) = make_float2(M, 1.0f / L);
 }
 
-template <int HD, bool K8, bool FINE>
-__global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedPlan p,
+template <int HD, bool K8, int NR>   // NR: column tiles of 8 query rows
+__global__ void __launch_bounds__(PGeo<HD, K8>::kThreads, 1) paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedPlan p,
                                                                    const int32_t* __restrict__ tables, const __half* __restrict__ q16, const PagedOut o, const __half* __restrict__ ksc, const __half* __restrict__ vsc,
                                                                    float* scores, float* scratch_o, float* scratch_ml, int32_t* counters, int32_t* err) {
-    using G = PGeo<HD, K8, FINE>; constexpr int kStages = G::kStages, kTile = G::kTile, NK = G::kNK, NT = 2 * NK;
+    using G = PGeo<HD, K8>; constexpr int kStages = G::kStages, kTile = G::kTile, NK = G::kNK;
     if (threadIdx.x == 0) { prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
     extern __shared__ __align__(128) uint8_t smem[];
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, ring = w & 3, h = w >> 2, g = lane >> 2, t4 = lane & 3;   // h = 0 score warp, 1 and 2 value warps, 3 producer
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, h = w >> 2, ring = (h == 3 && !K8) ? lane & 3 : w & 3, g = lane >> 2, t4 = lane & 3;   // h = 0 score warp, 1 and 2 value warps, 3 producer
+    const bool issues = h == 3 && (K8 ? lane == 0 : lane < kRings);
     const uint32_t sm_base = smem_u32(smem), bars = sm_base + G::kOffBars + ring * kMaxStages * 8, ebars = bars + kOffEBars;
     const uint32_t stage_off = ((sm_base + G::kOffStages + 1023u) & ~1023u) - sm_base, ring_stage0 = sm_base + stage_off + ring * G::kRingBytes;
     const uint32_t pfull = sm_base + G::kOffBars + kOffPBars + ring * 16, pempty = pfull + kRings * 16;
@@ -257,9 +295,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
     __syncthreads();
     pdl_wait(); pdl_launch_dependents();   // the set-up above overlapped the previous kernel's tail; nothing it wrote is read before this
 
-    const int kvh_n = p.kv_heads, rows = p.group * p.T, srow = rows <= 8 ? 8 : 16, mask = (1 << p.page_shift) - 1;
+    const int kvh_n = p.kv_heads, rows = p.group * p.T, srow = NR * 8, mask = (1 << p.page_shift) - 1;
     int tile = plan_first_tile(p, blockIdx.x); const int tile_end = plan_first_tile(p, blockIdx.x + 1);
-    int b = 0; uint32_t it = 0; bool dead = false;   // it: tiles this ring has consumed so far
+    int b = 0; uint32_t it = 0; bool dead = false;   // it: tiles this ring has worked on so far
 
     while (tile < tile_end) {
         while (p.tile_start[b + 1] <= tile) b++;
@@ -269,153 +307,168 @@ __global__ void __launch_bounds__(kThreads, 1) paged_decode_kernel(const __grid_
         const int32_t* table = tables + (int64_t)p.seq[b] * p.width;
         const int n_mine = n_here > ring ? (n_here - ring + kRings - 1) / kRings : 0;   // this ring's tiles: lt0 + ring, lt0 + ring + 4, ...
         const uint32_t it_seg = it;
-        ScoreState ss; ValueStateT<HD / 16> vst; vst.clear();
-        const int r0t = g / p.group, r1t = (g + 8) / p.group;
-        const int lim0 = g < rows ? kend - p.T + 1 + r0t : 0, lim1 = g + 8 < rows ? kend - p.T + 1 + r1t : 0;   // rows g and g + 8 see slots below these (never, when 0 or less)
-
-        // ---- producer: lane r serves ring r; page numbers are read three tiles ahead
-        int32_t pgA[2], pgB[2], pgC[2];
-        auto slot_of = [&](int i, int x) { return (lt0 + lane + i * kRings) * kTile + x * 16 * p.groups_per_box; };
-        auto load_pages = [&](int i, int32_t (&pg)[2]) {
-            pg[0] = __ldcg(table + (min(slot_of(i, 0), last) >> p.page_shift));
-            pg[1] = p.groups_per_box < NK ? __ldcg(table + (min(slot_of(i, 1), last) >> p.page_shift)) : 0;
-        };
-        const int nm = n_here > lane ? (n_here - lane + kRings - 1) / kRings : 0;
-        auto produce = [&](int i_from, int i_to) {
-            for (int i = i_from; i < min(i_to, nm); i++) {
-                const uint32_t cur = it + (uint32_t)i, sx = cur % kStages;
-                const uint32_t bar = sm_base + G::kOffBars + lane * kMaxStages * 8 + sx * 8, dst = sm_base + stage_off + lane * G::kRingBytes + sx * G::kStageBytes;
-                const int32_t pg[2] = {pgA[0], pgA[1]};
-                pgA[0] = pgB[0]; pgA[1] = pgB[1]; pgB[0] = pgC[0]; pgB[1] = pgC[1];
-                if (i + 3 < nm) load_pages(i + 3, pgC);
-                if (i >= kStages && !dead && !mbar_wait_bounded(bar + kOffEBars, ((cur / kStages) - 1u) & 1u, err)) { dead = true; atomicExch(err, 3); }
-                mbar_arrive_expect_tx(bar, (uint32_t)G::kStageBytes);
-#pragma unroll
-                for (int x = 0; x < NK; x++) {
-                    if (x && p.groups_per_box == NK) break;
-                    const int grp = (int)((p.layer_row0 + ((int64_t)pg[x] << p.page_shift) + (slot_of(i, x) & mask)) >> 4);
-                    tma_load_5d(dst + x * G::kGroupBytes, &tm_k, 0, 0, 0, grp, kvh, bar); tma_load_5d(dst + G::kHalfBytes + x * G::kGroupBytes, &tm_v, 0, 0, 0, grp, kvh, bar);
-                }
-            }
-        };
-        if (h == 3 && lane < kRings) {   // every stage is free here
-            if (nm > 0) load_pages(0, pgA);
-            if (nm > 1) load_pages(1, pgB);
-            if (nm > 2) load_pages(2, pgC);
-            produce(0, kStages);
-        }
-        // ---- int8 scales: lane j of the score warp fetches those of the tile's slot j, three tiles ahead, its page number three tiles before that
-        auto scale_slot = [&](int i) { return min((lt0 + ring + i * kRings) * kTile + (lane & (kTile - 1)), last); };
-        auto load_page1 = [&](int i) { return __ldcg(table + (scale_slot(i) >> p.page_shift)); };
-        auto load_scales = [&](int i, int32_t pg, uint32_t& ks, uint32_t& vs) {
-            const int64_t at = (((int64_t)pg << p.page_shift) + (scale_slot(i) & mask)) * kvh_n + kvh;   // ksc, vsc: this layer's planes
-            ks = __ldcg(reinterpret_cast<const unsigned short*>(ksc) + at); vs = __ldcg(reinterpret_cast<const unsigned short*>(vsc) + at);
-        };
-        uint32_t kA = 0, kB = 0, kC = 0, vA = 0, vB = 0, vC = 0; int32_t gD = 0, gE = 0, gF = 0;
-        if (K8 && h == 0 && n_mine > 0) {   // tiles past the end repeat the last slot: harmless, and the loads need no guards
-            const int32_t g0 = load_page1(0), g1 = load_page1(1), g2 = load_page1(2); gD = load_page1(3); gE = load_page1(4); gF = load_page1(5);
-            load_scales(0, g0, kA, vA); load_scales(1, g1, kB, vB); load_scales(2, g2, kC, vC);
-        }
-        // ---- the 16-row query block (rows t * group + j, zero behind the last)
-        for (int ch = tid; ch < 16 * (HD / 8); ch += kThreads) {
-            const int r = ch / (HD / 8), c16 = ch % (HD / 8); uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < rows) { const int t = r / p.group, j = r - t * p.group; v = *reinterpret_cast<const uint4*>(q16 + (((int64_t)b * p.tok_stride + p.tok0 + t) * (kvh_n * p.group) + kvh * p.group + j) * HD + c16 * 8); }
-            stage_q_chunk<K8>(smem + r * G::kQStride, c16, v);
-        }
-        __syncthreads();
-        if (K8 && !FINE) {   // row sums of the query block, for the bias of the codes
-            for (int r = w; r < 16; r += kWarps) {
-                float a = 0.0f;
-                for (int c = lane; c < HD / 8; c += 32) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(smem + r * G::kQStride + c * 16); const __half2* hp = reinterpret_cast<const __half2*>(&v);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) { const float2 f = __half22float2(hp[e]); a += f.x + f.y; }
-                }
-#pragma unroll
-                for (int off = 16; off >= 1; off >>= 1) a += __shfl_xor_sync(0xffffffffu, a, off);
-                if (lane == 0) reinterpret_cast<float*>(smem + G::kOffQsum)[r] = a;
-            }
-            __syncthreads();
-        }
-        const float qs[2] = {(K8 && !FINE) ? reinterpret_cast<const float*>(smem + G::kOffQsum)[g] : 0.0f, (K8 && !FINE) ? reinterpret_cast<const float*>(smem + G::kOffQsum)[g + 8] : 0.0f};
+        const int all_see = kend - p.T + 1;   // slots below this are seen by every row (columns that hold no query too: nobody reads what they get)
 
         if (h == 3) {
-            if (lane < kRings) { produce(kStages, 1 << 30); it += (uint32_t)nm; }   // 'it' of producer lane r counts ring r's tiles
-            __syncwarp();
-        } else if (h == 0) {
-            for (int i = 0; i < n_mine; i++) {
-                const uint32_t cur = it_seg + (uint32_t)i, stg = cur % kStages, par = (cur / kStages) & 1u, slot = cur & 1u;
-                const int key0 = (lt0 + ring + i * kRings) * kTile;
-                const uint32_t k_cur = kA, v_cur = vA; kA = kB; kB = kC; vA = vB; vB = vC;
-                if (K8 && i + 3 < n_mine) { const int32_t pg = gD; gD = gE; gE = gF; gF = load_page1(i + 6); load_scales(i + 3, pg, kC, vC); }
-                // a wait that runs out is recorded once; afterwards waits are skipped, the control flow and every arrival stay as they are
-                if (!dead && !mbar_wait_bounded(bars + stg * 8, par, err)) { dead = true; atomicExch(err, 1); }
-                float ks[NT][2], vs[NT][2];
+            // ---- producer: brings in the ring's tiles, refilling a stage as soon as its three warps have released it; page numbers are read three tiles
+            // ahead. int8: lane j also fetches the K and V scale of slot j, three tiles ahead (under load a request takes as long as all that is in flight before it), the page number of
+            // that three tiles earlier still, and stores it before the tile's copy is issued. Unrolled by three so that every load has registers of its own.
+            int32_t pg[3][2], spg[3]; unsigned short sc8[3][2];
+            auto first_slot = [&](int i) { return (lt0 + ring + i * kRings) * kTile; };
+            auto load_pages = [&](int i, int32_t (&x)[2]) {
+                x[0] = __ldcg(table + (min(first_slot(i), last) >> p.page_shift));
+                x[1] = p.groups_per_box < NK ? __ldcg(table + (min(first_slot(i) + 16, last) >> p.page_shift)) : 0;
+            };
+            auto scale_slot = [&](int i) { return min(first_slot(i) + lane, last); };   // slots behind the last repeat it: finite scales, and probabilities 0
+            auto scale_page = [&](int i) { return __ldcg(table + (scale_slot(i) >> p.page_shift)); };
+            auto load_scales = [&](int i, int32_t page, unsigned short (&x)[2]) {
+                const int64_t at = (((int64_t)page << p.page_shift) + (scale_slot(i) & mask)) * kvh_n + kvh;   // ksc, vsc: this layer's planes
+                x[0] = __ldcg(reinterpret_cast<const unsigned short*>(ksc) + at); x[1] = __ldcg(reinterpret_cast<const unsigned short*>(vsc) + at);
+            };
+            if (issues) { load_pages(0, pg[0]); load_pages(1, pg[1]); load_pages(2, pg[2]); }
+            if (K8) {
 #pragma unroll
-                for (int q = 0; q < 4 * NK; q++) {
-                    const int src = 8 * (q >> 1) + 2 * t4 + (q & 1);
-                    ks[q >> 1][q & 1] = K8 ? __half2float(__ushort_as_half((unsigned short)__shfl_sync(0xffffffffu, k_cur, src))) : 1.0f;
-                    vs[q >> 1][q & 1] = K8 ? __half2float(__ushort_as_half((unsigned short)__shfl_sync(0xffffffffu, v_cur, src))) : 1.0f;
-                }
-                float s[NT][4], pr[NT][4], al0, al1;
-                paged_scores<HD, K8, FINE>(sm_base, ring_stage0 + stg * G::kStageBytes, key0, lim0, lim1, ks, qs, lane, s);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(ebars + stg * 8);   // K of this stage is no longer needed
-                paged_softmax<NT, G::kPShift>(s, ss, pr, al0, al1);
-                if (scores) {   // [tile of the list][slot][8 or 16 rows]: full 32-byte sectors
-                    float* st = scores + ((int64_t)(tile + ring + i * kRings) * kTile + 2 * t4) * srow + g;
+                for (int j = 0; j < 3; j++) spg[j] = scale_page(j);
 #pragma unroll
-                    for (int nt8 = 0; nt8 < NT; nt8++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) { st[(8 * nt8 + e) * srow] = s[nt8][e]; if (srow == 16) st[(8 * nt8 + e) * 16 + 8] = s[nt8][2 + e]; }
-                }
-                if (K8) {
-#pragma unroll
-                    for (int q = 0; q < NT; q++) { pr[q][0] *= vs[q][0]; pr[q][1] *= vs[q][1]; pr[q][2] *= vs[q][0]; pr[q][3] *= vs[q][1]; }
-                }
-                if (cur >= 2 && !dead && !mbar_wait_bounded(pempty + slot * 8, ((cur >> 1) - 1u) & 1u, err)) { dead = true; atomicExch(err, 4); }
-                paged_publish<HD, K8, FINE>(sm_base + p_off + slot * G::kPBytes, reinterpret_cast<float*>(smem + p_off + (slot + 1) * G::kPBytes - 64), pr, al0, al1, lane);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(pfull + slot * 8);
+                for (int j = 0; j < 3; j++) { load_scales(j, spg[j], sc8[j]); spg[j] = scale_page(j + 3); }
             }
-            ss.l0 += __shfl_xor_sync(0xffffffffu, ss.l0, 1); ss.l0 += __shfl_xor_sync(0xffffffffu, ss.l0, 2);
-            ss.l1 += __shfl_xor_sync(0xffffffffu, ss.l1, 1); ss.l1 += __shfl_xor_sync(0xffffffffu, ss.l1, 2);
-            if (t4 == 0) { sm_ml[(ring * 16 + g) * 2] = ss.m0; sm_ml[(ring * 16 + g) * 2 + 1] = ss.l0; sm_ml[(ring * 16 + g + 8) * 2] = ss.m1; sm_ml[(ring * 16 + g + 8) * 2 + 1] = ss.l1; }
-        } else {
-            const int vh = h - 1;
-            for (int i = 0; i < n_mine; i++) {
-                const uint32_t cur = it_seg + (uint32_t)i, stg = cur % kStages, par = (cur / kStages) & 1u, slot = cur & 1u;
-                const uint32_t vt = ring_stage0 + stg * G::kStageBytes + G::kHalfBytes;
-                const int key0 = (lt0 + ring + i * kRings) * kTile;
-                if (!dead && !mbar_wait_bounded(bars + stg * 8, par, err)) { dead = true; atomicExch(err, 1); }
-                if (!K8 && key0 + kTile > kend) {   // the V rows behind the last slot become zeros (0 x NaN is not 0; int8 codes are finite whatever they are)
-                    const int nk = max(0, kend - key0);
-                    constexpr int kHC = G::kRowBytes / 32;   // 16-byte chunks of half a head row
-                    for (int idx = lane; idx < (kTile - nk) * kHC; idx += 32) {
-                        const int r = nk + idx / kHC, c = vh * kHC + idx % kHC;
-                        *reinterpret_cast<uint4*>(smem + (vt - sm_base) + (r >> 4) * G::kGroupBytes + (c >> 3) * 2048 + (r & 15) * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+            for (int i0 = 0; i0 < n_mine; i0 += 3)
+#pragma unroll
+                for (int j = 0; j < 3; j++) {
+                    const int i = i0 + j;
+                    if (i >= n_mine) break;
+                    const uint32_t cur = it + (uint32_t)i, sx = cur % kStages, bar = bars + sx * 8, dst = ring_stage0 + sx * G::kStageBytes;
+                    if (issues && i >= kStages && !dead && !mbar_wait_bounded(ebars + sx * 8, ((cur / kStages) - 1u) & 1u, err)) { dead = true; atomicExch(err, 3); }
+                    if (K8) {
+                        __syncwarp();
+                        reinterpret_cast<uint32_t*>(smem + G::kOffScale)[(ring * kStages + sx) * 32 + lane] = (uint32_t)sc8[j][0] | (uint32_t)sc8[j][1] << 16;
+                        __syncwarp();   // the arrival below publishes them
                     }
-                    fence_proxy_async();   // generic writes to a stage that TMA fills again
-                    __syncwarp();
+                    if (issues) {
+                        mbar_arrive_expect_tx(bar, (uint32_t)G::kStageBytes);
+#pragma unroll
+                        for (int x = 0; x < NK; x++) {
+                            if (x && p.groups_per_box == NK) break;
+                            const int grp = (int)((p.layer_row0 + ((int64_t)pg[j][x] << p.page_shift) + ((first_slot(i) + 16 * x) & mask)) >> 4);
+                            tma_load_5d(dst + x * G::kGroupBytes, &tm_k, 0, 0, 0, grp, kvh, bar); tma_load_5d(dst + G::kHalfBytes + x * G::kGroupBytes, &tm_v, 0, 0, 0, grp, kvh, bar);
+                        }
+                        load_pages(i + 3, pg[j]);   // behind the ring's last tile: the last page again
+                    }
+                    if (K8) { load_scales(i + 3, spg[j], sc8[j]); spg[j] = scale_page(i + 6); }
                 }
-                if (!dead && !mbar_wait_bounded(pfull + slot * 8, (cur >> 1) & 1u, err)) { dead = true; atomicExch(err, 5); }
-                paged_values<HD, K8, FINE>(vt, sm_base + p_off + slot * G::kPBytes, reinterpret_cast<const float*>(smem + p_off + (slot + 1) * G::kPBytes - 64), vst, lane, vh);
-                __syncwarp();
-                if (lane == 0) { mbar_arrive(pempty + slot * 8); mbar_arrive(ebars + stg * 8); }
+        } else {
+            // ---- the query block (rows t * group + j, zero behind the last; int8: columns permuted inside each 16-dim block)
+            for (int ch = tid; ch < NR * 8 * (HD / 8); ch += 384) {
+                const int r = ch / (HD / 8), c16 = ch % (HD / 8); uint4 v = make_uint4(0, 0, 0, 0);
+                if (r < rows) { const int t = r / p.group, j = r - t * p.group; v = *reinterpret_cast<const uint4*>(q16 + (((int64_t)b * p.tok_stride + p.tok0 + t) * (kvh_n * p.group) + kvh * p.group + j) * HD + c16 * 8); }
+                stage_q_chunk<K8>(smem + r * G::kQStride, c16, v);
             }
-            if (K8 && !FINE) vst.finish_bias(kI8Bias);
+            asm volatile("bar.sync 1, 384;" ::: "memory");   // the twelve score and value warps: the producers are under way already
+
+            if (h == 0) {
+                RowsState<NR> ss; int lim[NR][2]; uint32_t qf[HD / 16][2];
+#pragma unroll
+                for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) { const int r = nr * 8 + 2 * t4 + e; ss.m[nr][e] = -INFINITY; ss.l[nr][e] = 0.0f; lim[nr][e] = r < rows ? kend - p.T + 1 + r / p.group : 0; }   // the row sees slots below this (none, when 0 or less)
+                if (NR == 1) {
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; kk += 2) q_frags(sm_base, G::kQStride, 0, kk, lane, qf[kk], qf[kk + 1]);
+                }
+                for (int i = 0; i < n_mine; i++) {
+                    const uint32_t cur = it_seg + (uint32_t)i, stg = cur % kStages, par = (cur / kStages) & 1u, slot = cur & 1u;
+                    const int key0 = (lt0 + ring + i * kRings) * kTile;
+                    // a wait that runs out is recorded once; afterwards waits are skipped, the control flow and every arrival stay as they are
+                    if (!dead && !mbar_wait_bounded(bars + stg * 8, par, err)) { dead = true; atomicExch(err, 1); }
+                    uint32_t sc[NK][2]; float ks[NK][2];   // K scale in the low half, V scale in the high half, of slots 16 * sb + g and 8 further
+#pragma unroll
+                    for (int sb = 0; sb < NK; sb++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            if (K8) sc[sb][e] = *reinterpret_cast<const uint32_t*>(smem + G::kOffScale + (ring * kStages + stg) * 128 + (16 * sb + 8 * e + g) * 4);
+                            ks[sb][e] = K8 ? __half2float(__ushort_as_half((unsigned short)sc[sb][e])) : 1.0f;
+                        }
+                    float s[NK][NR][4], al[NR][2];
+                    paged_scores<HD, K8, NR>(sm_base, ring_stage0 + stg * G::kStageBytes, qf, ks, lane, s);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(ebars + stg * 8);   // K and the scales (in registers by now) of this stage are no longer needed
+                    if (key0 + kTile > all_see) {   // masked by select: what lies behind the last slot may be anything
+#pragma unroll
+                        for (int sb = 0; sb < NK; sb++)
+#pragma unroll
+                            for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) if (key0 + 16 * sb + 8 * (e >> 1) + g >= lim[nr][e & 1]) s[sb][nr][e] = -INFINITY;
+                    }
+                    if (scores) {   // [tile of the list][slot][8 or 16 rows]: full 32-byte sectors
+                        float* st = scores + ((int64_t)(tile + ring + i * kRings) * kTile + g) * srow + 2 * t4;
+#pragma unroll
+                        for (int sb = 0; sb < NK; sb++)
+#pragma unroll
+                            for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                                for (int e = 0; e < 2; e++) *reinterpret_cast<float2*>(st + (16 * sb + 8 * e) * srow + nr * 8) = make_float2(s[sb][nr][2 * e], s[sb][nr][2 * e + 1]);
+                    }
+                    paged_softmax<NK, NR, G::kPShift>(s, ss, al);
+                    if (K8) {
+#pragma unroll
+                        for (int sb = 0; sb < NK; sb++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const float v = __half2float(__ushort_as_half((unsigned short)(sc[sb][e >> 1] >> 16)));
+#pragma unroll
+                                for (int nr = 0; nr < NR; nr++) s[sb][nr][e] *= v;
+                            }
+                    }
+                    if (cur >= 2 && !dead && !mbar_wait_bounded(pempty + slot * 8, ((cur >> 1) - 1u) & 1u, err)) { dead = true; atomicExch(err, 4); }
+                    paged_publish<HD, K8, NR>(sm_base + p_off + slot * G::kPBytes, reinterpret_cast<float*>(smem + p_off + (slot + 1) * G::kPBytes - 64), s, al, p.two_terms, lane);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(pfull + slot * 8);
+                }
+#pragma unroll
+                for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float l = ss.l[nr][e];
+                        l += __shfl_xor_sync(0xffffffffu, l, 4); l += __shfl_xor_sync(0xffffffffu, l, 8); l += __shfl_xor_sync(0xffffffffu, l, 16);
+                        if (g == 0) *reinterpret_cast<float2*>(sm_ml + (ring * 16 + nr * 8 + 2 * t4 + e) * 2) = make_float2(ss.m[nr][e], l);
+                    }
+            } else {
+                const int vh = h - 1; ValueAcc<HD, NR> vst; vst.clear();
+                for (int i = 0; i < n_mine; i++) {
+                    const uint32_t cur = it_seg + (uint32_t)i, stg = cur % kStages, par = (cur / kStages) & 1u, slot = cur & 1u;
+                    const uint32_t vt = ring_stage0 + stg * G::kStageBytes + G::kHalfBytes;
+                    const int key0 = (lt0 + ring + i * kRings) * kTile;
+                    if (!dead && !mbar_wait_bounded(bars + stg * 8, par, err)) { dead = true; atomicExch(err, 1); }
+                    if (!K8 && key0 + kTile > kend) {   // the V rows behind the last slot become zeros (0 x NaN is not 0; int8 codes are finite whatever they are)
+                        const int nk = max(0, kend - key0);
+                        constexpr int kHC = G::kRowBytes / 32;   // 16-byte chunks of half a head row
+                        for (int idx = lane; idx < (kTile - nk) * kHC; idx += 32) {
+                            const int r = nk + idx / kHC, c = vh * kHC + idx % kHC;
+                            *reinterpret_cast<uint4*>(smem + (vt - sm_base) + (r >> 4) * G::kGroupBytes + (c >> 3) * 2048 + (r & 15) * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async();   // generic writes to a stage that TMA fills again
+                        __syncwarp();
+                    }
+                    if (!dead && !mbar_wait_bounded(pfull + slot * 8, (cur >> 1) & 1u, err)) { dead = true; atomicExch(err, 5); }
+                    const float* alpha = reinterpret_cast<const float*>(smem + p_off + (slot + 1) * G::kPBytes - 64);
+                    if (!K8 || p.two_terms) paged_values<HD, K8, NR, true>(vt, sm_base + p_off + slot * G::kPBytes, alpha, vst, lane, vh); else paged_values<HD, K8, NR, false>(vt, sm_base + p_off + slot * G::kPBytes, alpha, vst, lane, vh);
+                    __syncwarp();
+                    if (lane == 0) { mbar_arrive(pempty + slot * 8); mbar_arrive(ebars + stg * 8); }
+                }
+                asm volatile("bar.sync %0, 64;" ::"r"(2 + ring) : "memory");   // both value warps are done with the ring's stages (and so is the score warp, whose last P they have used): the rows of O go there
+                float* mo = reinterpret_cast<float*>(smem + stage_off + ring * G::kRingBytes);
+#pragma unroll
+                for (int j = 0; j < HD / 32; j++)
+#pragma unroll
+                    for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) mo[(nr * 8 + 2 * t4 + (e & 1)) * G::kMergeStride + vh * (HD / 2) + 16 * j + (K8 ? 2 * g + (e >> 1) : g + 8 * (e >> 1))] = vst.o[j][nr][e];
+            }
         }
-        if (h != 3) it = it_seg + (uint32_t)n_mine;
+        it = it_seg + (uint32_t)n_mine;
 
         // ---- join the four rings (every tile issued has been waited for: no copy is in flight)
-        __syncthreads();
-        if (h == 1 || h == 2) {
-            float* mo = reinterpret_cast<float*>(smem + stage_off + ring * G::kRingBytes);
-#pragma unroll
-            for (int j = 0; j < HD / 16; j++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) { const int d = (h - 1) * (HD / 2) + dim_of<K8>(j, c, t4); mo[g * G::kMergeStride + d] = vst.o[j][c]; mo[(g + 8) * G::kMergeStride + d] = vst.o[j][2 + c]; }
-        }
         __syncthreads();
         constexpr int kTpr = HD / 2, kRowPar = 384 / kTpr;   // threads per row (two dims each), rows at a time over the twelve ring warps
         const int seg = b * kvh_n + kvh, c_first = plan_cta_of_tile(p, seg_first), n_contrib = plan_cta_of_tile(p, seg_end - 1) - c_first + 1;
@@ -501,7 +554,7 @@ __global__ void __launch_bounds__(1024) paged_combine_kernel(const __grid_consta
 }
 
 // weight[kv head][slot] += sum over the rows of 2^(s * log2 e - m + shift) / l: the slot's final probabilities, from the scores the decode kernel
-// kept and the joined (m, l). A thread per (slot, KV head) in the order of the tile list: 32 (or 64) contiguous bytes per thread, nothing shared, no atomics.
+// kept and the joined (m, 1 / l). A thread per (slot, KV head) in the order of the tile list: 32 (or 64) contiguous bytes per thread, nothing shared, no atomics.
 __global__ void __launch_bounds__(256) paged_weight_kernel(const __grid_constant__ PagedPlan p, const int32_t* __restrict__ tables, const float* __restrict__ scores, const float* __restrict__ fin_ml,
                                                            float* __restrict__ weight /* the layer's plane [page][kv head][slot] */, const int tile_shift, const float shift) {
     pdl_wait(); pdl_launch_dependents();
@@ -520,7 +573,7 @@ __global__ void __launch_bounds__(256) paged_weight_kernel(const __grid_constant
         for (int e = 0; e < 4; e++) {
             if (r4 + e >= rows) break;
             const float2 m = __ldcg(ml + r4 + e);
-            if (x[e] != -INFINITY) sum += ex2(fmaf(x[e], kLog2e, shift - m.x)) / m.y;   // a masked slot adds nothing (its row may have no maximum at all)
+            if (x[e] != -INFINITY) sum += ex2(fmaf(x[e], kLog2e, shift - m.x)) * m.y;   // a masked slot adds nothing (its row may have no maximum at all)
         }
     }
     const int page = __ldcg(tables + (int64_t)p.seq[b] * p.width + (slot >> p.page_shift));
@@ -552,28 +605,28 @@ int paged_tile_keys(const PagedCtx& c) { return (c.cfg.head_dim == 256 && !c.int
 size_t paged_part_floats(const PagedCtx& c) { return (size_t)(c.sm_count + KATA_PAGED_MAX_BATCH * c.cfg.kv_heads) * 16 * c.cfg.head_dim; }
 size_t paged_part_ml_floats(const PagedCtx& c) { return (size_t)(c.sm_count + KATA_PAGED_MAX_BATCH * c.cfg.kv_heads) * 32; }
 
-#define KATA_PAGED_KERNELS(X) X(256, false, false) X(256, false, true) X(256, true, false) X(256, true, true) X(128, false, false) X(128, false, true) X(128, true, false) X(128, true, true)
+#define KATA_PAGED_KERNELS(X) X(256, false, 1) X(256, false, 2) X(256, true, 1) X(256, true, 2) X(128, false, 1) X(128, false, 2) X(128, true, 1) X(128, true, 2)
 
 cudaError_t configure_paged_decode(const PagedCtx& c) {   // shared-memory opt-in, per device
     cudaError_t e = cudaSuccess;
-#define X(HD, K8, FINE) if (e == cudaSuccess && c.cfg.head_dim == HD && c.int8() == K8) e = cudaFuncSetAttribute(paged_decode_kernel<HD, K8, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, PGeo<HD, K8, FINE>::kSmem);
+#define X(HD, K8, NR) if (e == cudaSuccess && c.cfg.head_dim == HD && c.int8() == K8) e = cudaFuncSetAttribute(paged_decode_kernel<HD, K8, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, PGeo<HD, K8>::kSmem);
     KATA_PAGED_KERNELS(X)
 #undef X
     return e;
 }
 
 cudaError_t launch_paged_decode(PagedCtx& c, int layer, int n, const int32_t* seq, const int32_t* n_slots, int T, const __half* q16, const float* gate, void* out, int out_dtype, bool accumulate, cudaStream_t s) {
-    const int per_pass = std::max(1, 16 / c.group), tile_keys = paged_tile_keys(c), hd = c.cfg.head_dim; const bool fine = out_dtype == KATA_ACT_F32;
+    const int per_pass = std::max(1, 16 / c.group), tile_keys = paged_tile_keys(c), hd = c.cfg.head_dim;
     for (int t0 = 0; t0 < T; t0 += per_pass) {   // each pass is independent: all rows are in the cache, token t of the call sees slots below n_slots - T + 1 + t
         PagedPlan p{}; p.n = n; p.T = std::min(per_pass, T - t0); p.group = c.group; p.kv_heads = c.cfg.kv_heads; p.tok_stride = T; p.tok0 = t0;
-        p.page_shift = c.page_shift; p.width = c.width; p.groups_per_box = c.box_groups; p.layer_row0 = (int64_t)layer * c.rows_per_layer;
+        p.two_terms = !c.int8() || out_dtype == KATA_ACT_F32; p.page_shift = c.page_shift; p.width = c.width; p.groups_per_box = c.box_groups; p.layer_row0 = (int64_t)layer * c.rows_per_layer;
         for (int i = 0; i < n; i++) { p.seq[i] = seq[i]; p.kend[i] = std::max(0, n_slots[i] - T + t0 + p.T); }
         split_paged_tiles(p, tile_keys, c.sm_count);
         // a pass's limits are kend - p.T + 1 + t: where kend was raised to 0 they are 0 or less, as they should be
         const PagedOut o{gate, out, out_dtype, accumulate ? c.fin_ml : nullptr}; float* scores = accumulate ? c.scores : nullptr;
         if (accumulate && p.tile_start[n] > c.score_tiles) return cudaErrorInvalidValue;   // cannot be: the pool bounds the tiles
         cudaError_t e = cudaErrorInvalidValue;
-#define X(HD, K8, FINE) if (hd == HD && c.int8() == K8 && fine == FINE) e = launch_pdl(paged_decode_kernel<HD, K8, FINE>, dim3(p.n_ctas), dim3(kThreads), PGeo<HD, K8, FINE>::kSmem, s, c.tm_k, c.tm_v, p, (const int32_t*)c.d_table, q16, o, \
+#define X(HD, K8, NR) if (hd == HD && c.int8() == K8 && (c.group * p.T > 8) == (NR == 2)) e = launch_pdl(paged_decode_kernel<HD, K8, NR>, dim3(p.n_ctas), dim3(PGeo<HD, K8>::kThreads), PGeo<HD, K8>::kSmem, s, c.tm_k, c.tm_v, p, (const int32_t*)c.d_table, q16, o, \
             (const __half*)c.layer_plane(KATA_PAGED_K_SCALE, layer), (const __half*)c.layer_plane(KATA_PAGED_V_SCALE, layer), scores, c.part_o, c.part_ml, c.counters, c.d_err);
         KATA_PAGED_KERNELS(X)
 #undef X
@@ -588,7 +641,7 @@ cudaError_t launch_paged_decode(PagedCtx& c, int layer, int n, const int32_t* se
         if (accumulate) {
             const int64_t keys = (int64_t)p.tile_start[n] * tile_keys;
             e = launch_pdl(paged_weight_kernel, dim3((unsigned)((keys + 255) / 256)), dim3(256), 0, s, p, (const int32_t*)c.d_table, (const float*)c.scores, (const float*)c.fin_ml, (float*)c.layer_plane(KATA_PAGED_WEIGHT, layer),
-                           tile_keys == 16 ? 4 : 5, c.int8() ? (float)PGeo<256, true, false>::kPShift : (float)PGeo<256, false, false>::kPShift);
+                           tile_keys == 16 ? 4 : 5, c.int8() ? (float)PGeo<256, true>::kPShift : (float)PGeo<256, false>::kPShift);
             if (e != cudaSuccess) return e;
             c.launches++;
         }
