@@ -17,7 +17,8 @@ int pfail(PagedCtx& c, int code, const char* fmt, ...) {
     try { c.err = buf; } catch (const std::exception&) {}
     return code;
 }
-int pcuda(PagedCtx& c, cudaError_t e, const char* what) { return pfail(c, KATA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e)); }
+int pcuda(PagedCtx& c, cudaError_t e, const char* what) { cudaGetLastError();   // reported here: not again by the next call
+    return pfail(c, KATA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e)); }
 
 struct DeviceGuard {
     int prev = -1;

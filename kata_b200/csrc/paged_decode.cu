@@ -43,7 +43,7 @@ constexpr int kOffEBars = kRings * kMaxStages * 8, kOffPBars = 2 * kOffEBars, kB
 
 template <int HD, bool K8> struct PGeo {
     static constexpr int kThreads = (3 * kRings + (K8 ? kRings : 1)) * 32;               // fp16: one producer warp, lane r for ring r (in step: 142 us for eight sequences of 16K to 32K slots, 154 with one per ring); int8: one per ring
-    static constexpr int kRowBytes = HD * (K8 ? 1 : 2), kNB = kRowBytes / 128;           // bytes and 128-byte column blocks of a head row
+    static constexpr int kRowBytes = HD * (K8 ? 1 : 2);                                  // bytes of a head row
     static constexpr int kNK = (HD == 256 && !K8) ? 1 : 2, kTile = 16 * kNK;             // 16-slot groups and slots per tile
     static constexpr int kGroupBytes = 16 * kRowBytes, kHalfBytes = kNK * kGroupBytes;   // K (or V) of one group, of one tile
     static constexpr int kStageBytes = 2 * kHalfBytes, kStages = kStageBytes == 16384 ? 3 : 6;

@@ -3,18 +3,31 @@
 // Slots kept below `keep` stay where they are; the i-th kept slot at or behind `keep` moves into the i-th free slot below it. Every row that moves is read
 // behind `keep` and written below it, so no order of the copies can clobber one, and as few rows move as can.
 //
-// select: one CTA per (layer, sequence, KV head). Weights as order-preserving 32-bit integers, kept in shared memory when they fit; the keep-th largest by a radix select over digits of
-// 11, 11 and 10 bits; then bit masks of the slots (32 per word) with prefix sums per word give every free slot its rank and every rank its mover.
+// select, up to 5,120 slots: one CTA per (layer, sequence, KV head) with the slots' keys (weights as order-preserving 32-bit integers) in registers. The keep-th largest bit by bit from
+// the top, a count over the block per bit (some 330 clocks), ended early once a count is `keep` (histograms of digits in shared memory were slower: their atomics take a
+// clock per lane); then the words of 32 slots get their prefix sums by ballots and shuffles, the movers go to a list in shared memory in order, and every free slot
+// takes the mover of its rank.
+// select_cluster, above that: eight CTAs with a contiguous eighth of the slots each (one SM needs 12 us for the loads of 32K slots alone). Up to 131,072 slots the keys are in registers, and the
+// threshold is found by bounds: a sample of 512 keys gives two values that it hardly lies outside of (three standard deviations), the keys between them are gathered through distributed
+// shared memory, narrowed by a second sample and searched by one warp. Where the counts do not confirm the bounds, or too many keys lie between (one value shared
+// by many slots), and for longer sequences, whose keys are read again in every pass, a radix select over the cluster's summed histograms finds it. Ranks of free slots and movers come
+// from prefix sums per word; the free slots are listed by rank where they lie, and each mover looks its own up.
 // move: a warp per 32 destinations, lanes agreeing by ballot on those that receive a row; each row is 16-byte copies of K and V. Bound by HBM: 2 x row bytes per move.
 #include <algorithm>
+#include <type_traits>
+
+#include <cooperative_groups.h>
 
 #include "paged_internal.cuh"
 
 namespace kata {
 namespace {
 
-constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32, kBins = 2048;
-constexpr int kSelSmemMax = 222 * 1024;
+constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32;
+constexpr int kSelOne = 10 * kSelThreads, kSelMany = 64;   // one CTA per (layer, sequence, KV head) up to so many slots, or (up to 32,768) when there are so many of them: 256 times 8,000 slots took 36 us
+                                                           // beside the move so, 180 us as clusters, whose latency then adds up
+constexpr int kSelCluster = 8, kCluSlots = kSelCluster * kSelThreads, kCluMax = 8 * kCluSlots;   // slots of a cluster per register of its threads; slots that it, or one CTA, selects from by bounds
+constexpr int kSample = kSelThreads, kOwn = 1024, kNear = 1024, kGather = 12;   // keys in a sample; keys that may lie between the bounds per CTA, after the second narrowing, and per thread of the gathered ones
 
 struct EvictArgs {
     int keep, sink, recent, width, page_shift, kv_heads, n, layer0;
@@ -22,114 +35,332 @@ struct EvictArgs {
     const int32_t* tables; float* weight; int32_t* age; int32_t* src;
 };
 
-__device__ __forceinline__ uint32_t order_key(float w) {   // larger float, larger integer; NaN below everything; -0 = +0
-    if (w != w) return 0u;
+__device__ __forceinline__ uint32_t order_key(float w) {   // larger float, larger integer; NaN below everything (1; 0 stands for no slot); -0 = +0
+    if (w != w) return 1u;
     const uint32_t u = __float_as_uint(w + 0.0f);
     return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-// exclusive prefix sums over x[0, n) in place, by the whole block; returns the total to every thread
-__device__ int block_exclusive_scan(int32_t* x, int n, int32_t* s_warp) {
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, per = (n + kSelThreads - 1) / kSelThreads, lo = min(tid * per, n), hi = min(lo + per, n);
-    int sum = 0;
-    for (int i = lo; i < hi; i++) sum += x[i];
-    int inc = sum;
+__device__ __forceinline__ int warp_inclusive(int v) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) { const int o = __shfl_up_sync(0xffffffffu, inc, off); if (lane >= off) inc += o; }
-    if (lane == 31) s_warp[w] = inc;
-    __syncthreads();
-    if (w == 0) {
-        int v = s_warp[lane];
+    for (int off = 1; off < 32; off <<= 1) { const int o = __shfl_up_sync(0xffffffffu, v, off); if (lane >= off) v += o; }
+    return v;
+}
+// c += k >= at, as a compare and a predicated add (the compiler's form of `c += k >= at` takes 8 clocks a key, this 4)
+__device__ __forceinline__ void add_if_ge(int& c, uint32_t k, uint32_t at) { asm("{\n .reg .pred p;\n setp.ge.u32 p, %1, %2;\n @p add.s32 %0, %0, 1;\n}" : "+r"(c) : "r"(k), "r"(at)); }
+
+// A value between lo and hi that at least `target` of a warp's keys reach: exactly so many, or it is the target-th largest key itself. All keys are at least lo (or 0: none).
+template <int N> __device__ __forceinline__ uint32_t warp_search(const uint32_t (&k)[N], int target, uint32_t lo, uint32_t hi) {
+    uint32_t v = lo == hi ? lo : lo & ~(0xffffffffu >> __clz(lo ^ hi));
+#pragma unroll 1
+    for (int bit = lo == hi ? -1 : 31 - __clz(lo ^ hi); bit >= 0; bit--) {
+        const uint32_t at = v | 1u << bit; int c[4] = {};
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) { const int o = __shfl_up_sync(0xffffffffu, v, off); if (lane >= off) v += o; }
-        s_warp[lane] = v;
+        for (int i = 0; i < N; i++) add_if_ge(c[i & 3], k[i], at);
+        const int n = __reduce_add_sync(0xffffffffu, (c[0] + c[1]) + (c[2] + c[3]));
+        if (n >= target) v = at;
+        if (n == target) break;
     }
+    return v;
+}
+__device__ __forceinline__ uint32_t evict_key(const EvictArgs& a, const int32_t* table, const float* weight, const int32_t* age, int kvh, int j, int newest) {   // of one slot
+    const int64_t at = (((int64_t)__ldcg(table + (j >> a.page_shift)) * a.kv_heads + kvh) << a.page_shift) + (j & ((1 << a.page_shift) - 1));
+    const int ag = __ldcg(age + at); const float wt = __ldcg(weight + at);
+    return (ag < a.sink || ag >= newest) ? 0xFF800000u : order_key(wt);   // 0xFF800000: the key of +inf
+}
+// the same for N slots of a thread, slot(i) clamped to the last: without branches, so that the requests are under way together, eight slots at a time
+template <int N, typename F> __device__ __forceinline__ void evict_keys(const EvictArgs& a, const int32_t* table, const float* weight, const int32_t* age, int kvh, int n_slots, int newest, F slot, uint32_t (&key)[N]) {
+    const int in_page = (1 << a.page_shift) - 1;
+#pragma unroll
+    for (int i = 0; i < N; i++) key[i] = (uint32_t)__ldcg(table + (min(slot(i), n_slots - 1) >> a.page_shift));
+#pragma unroll
+    for (int i0 = 0; i0 < N; i0 += 8) {
+        float wt[8]; int ag[8];
+#pragma unroll
+        for (int x = 0; x < 8; x++) if (i0 + x < N) {
+            const int64_t at = (((int64_t)(int32_t)key[i0 + x] * a.kv_heads + kvh) << a.page_shift) + (min(slot(i0 + x), n_slots - 1) & in_page);
+            wt[x] = __ldcg(weight + at); ag[x] = __ldcg(age + at);
+        }
+#pragma unroll
+        for (int x = 0; x < 8; x++) if (i0 + x < N) key[i0 + x] = slot(i0 + x) < n_slots ? ((ag[x] < a.sink || ag[x] >= newest) ? 0xFF800000u : order_key(wt[x])) : 0u;
+    }
+}
+// of a value per warp, the sum over the warps before this one; s: kSelWarps words, not in use
+__device__ __forceinline__ int warps_before(int32_t* s, int v) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    if (lane == 0) s[w] = v;
     __syncthreads();
-    int run = inc - sum + (w ? s_warp[w - 1] : 0); const int total = s_warp[kSelWarps - 1];
-    for (int i = lo; i < hi; i++) { const int c = x[i]; x[i] = run; run += c; }
-    __syncthreads();
-    return total;
+    return (int)__reduce_add_sync(0xffffffffu, lane < w ? s[lane] : 0);
 }
 
-// grid (kv heads, sequences, layers)
-__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_constant__ PagedBatch b, const __grid_constant__ EvictArgs a, const int words_cap, const int cached) {
-    extern __shared__ __align__(16) uint32_t dyn[];
-    uint32_t* kept = dyn; int32_t* pre_h = reinterpret_cast<int32_t*>(dyn + words_cap); int32_t* pre_m = pre_h + words_cap; uint32_t* keys = dyn + 3 * words_cap;   // keys: when cached
-    __shared__ int32_t hist[kBins]; __shared__ int32_t s_warp[kSelWarps]; __shared__ int s_bin, s_left;
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, kvh = blockIdx.x, bi = blockIdx.y, l = blockIdx.z, S = b.slot[bi], seen = b.age[bi], keep = a.keep;
+// grid (kv heads, sequences, layers). ITEMS: words of 32 slots per warp; warp w has words w * ITEMS .. and lane i (for more than 32: and i + 32) keeps what concerns word w * ITEMS + i
+template <int ITEMS>
+__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_constant__ PagedBatch b, const __grid_constant__ EvictArgs a) {
+    __shared__ uint16_t list[ITEMS * kSelThreads / 2];   // the movers in order: at most half of the slots
+    __shared__ int32_t s_n[2][kSelWarps], s_b[kSelWarps], s_c[kSelWarps], s_d[kSelWarps];
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, kvh = blockIdx.x, bi = blockIdx.y, l = blockIdx.z, S = b.slot[bi], keep = a.keep;
     pdl_wait(); pdl_launch_dependents();
     int32_t* src = a.src + (((int64_t)l * a.n + bi) * a.kv_heads + kvh) * keep;
     if (S <= keep) { for (int j = tid; j < keep; j += kSelThreads) src[j] = j < S ? j : -1; return; }
-    const int32_t* table = a.tables + (int64_t)b.seq[bi] * a.width; const float* weight = a.weight + (int64_t)(a.layer0 + l) * a.plane_stride; const int32_t* age = a.age + (int64_t)(a.layer0 + l) * a.plane_stride;
-    const int newest = seen - a.recent;   // ages from here on are protected
-    auto load_key = [&](int j) {
-        const int64_t at = (((int64_t)__ldcg(table + (j >> a.page_shift)) * a.kv_heads + kvh) << a.page_shift) + (j & ((1 << a.page_shift) - 1));
-        const int ag = __ldcg(age + at);
-        return (ag < a.sink || ag >= newest) ? 0xFF800000u : order_key(__ldcg(weight + at));   // 0xFF800000: the key of +inf
-    };
-    auto key_of = [&](int j) { return cached ? keys[j] : load_key(j); };
-    if (cached) for (int j = tid; j < S; j += kSelThreads) keys[j] = load_key(j);
-    // ---- the keep-th largest key
-    uint32_t prefix = 0, prefix_mask = 0; int left = keep;   // left: how many of the keys that match the prefix are kept
+    const int j0 = w * ITEMS * 32 + lane;   // slot of item i: j0 + 32 * i
+    uint32_t key[ITEMS];
+    evict_keys(a, a.tables + (int64_t)b.seq[bi] * a.width, a.weight + (int64_t)(a.layer0 + l) * a.plane_stride, a.age + (int64_t)(a.layer0 + l) * a.plane_stride, kvh, S, b.age[bi] - a.recent, [&](int i) { return j0 + 32 * i; }, key);
+    // ---- the keep-th largest key: the largest value that at least `keep` keys reach
+    uint32_t prefix = 0; int reach = S;   // keys >= prefix
 #pragma unroll 1
-    for (int pass = 0; pass < 3; pass++) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-        for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-        __syncthreads();
-        for (int j = tid; j < S; j += kSelThreads) { const uint32_t k = key_of(j); if ((k & prefix_mask) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1); }
-        __syncthreads();
-        // the bin, from the top, in which the count passes `left`: thread t owns bins 2t and 2t + 1 counted from the top
-        const int top0 = hist[kBins - 1 - 2 * tid], top1 = hist[kBins - 2 - 2 * tid]; int inc = top0 + top1;
+    for (int bit = 31; bit >= 0 && reach != keep; bit--) {
+        int c[2] = {};
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) { const int o = __shfl_up_sync(0xffffffffu, inc, off); if (lane >= off) inc += o; }
-        if (lane == 31) s_warp[w] = inc;
+        for (int i = 0; i < ITEMS; i++) add_if_ge(c[i & 1], key[i], prefix | 1u << bit);
+        int n = __reduce_add_sync(0xffffffffu, c[0] + c[1]);
+        if (lane == 0) s_n[bit & 1][w] = n;   // two rows in turn: one barrier per count
         __syncthreads();
-        if (w == 0) {
-            int v = s_warp[lane];
-#pragma unroll
-            for (int off = 1; off < 32; off <<= 1) { const int o = __shfl_up_sync(0xffffffffu, v, off); if (lane >= off) v += o; }
-            s_warp[lane] = v;
-        }
-        __syncthreads();
-        const int before = inc - top0 - top1 + (w ? s_warp[w - 1] : 0);   // keys in higher bins than this thread's
-        if (before < left && before + top0 >= left) { s_bin = kBins - 1 - 2 * tid; s_left = left - before; }
-        else if (before + top0 < left && before + top0 + top1 >= left) { s_bin = kBins - 2 - 2 * tid; s_left = left - before - top0; }
-        __syncthreads();
-        prefix |= (uint32_t)s_bin << shift; prefix_mask |= ((1u << bits) - 1) << shift; left = s_left;
-        __syncthreads();
+        n = __reduce_add_sync(0xffffffffu, lane < kSelWarps ? s_n[bit & 1][lane] : 0);
+        if (n >= keep) { prefix |= 1u << bit; reach = n; }
     }
-    // prefix is the keep-th largest key; of the slots that have it, the `left` lowest are kept
-    const int words = (S + 31) >> 5;
-    for (int wd = w; wd < words; wd += kSelWarps) {
-        const int j = wd * 32 + lane; const uint32_t k = j < S ? key_of(j) : 0u;
-        const uint32_t gt = __ballot_sync(0xffffffffu, j < S && k > prefix), eq = __ballot_sync(0xffffffffu, j < S && k == prefix);
-        if (lane == 0) { kept[wd] = gt; pre_h[wd] = (int32_t)eq; pre_m[wd] = __popc(eq); }
+    // ---- every key above prefix is kept; of those equal to it (all of them, when as many as `keep` reach it) the lowest
+    constexpr int WL = (ITEMS + 31) / 32;   // words per lane: w * ITEMS + lane and, 32 further, another
+    uint32_t gt[WL] = {}, eq[WL] = {};
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+        const uint32_t g = __ballot_sync(0xffffffffu, key[i] > prefix), e = __ballot_sync(0xffffffffu, key[i] == prefix);
+        if (lane == (i & 31)) { gt[i >> 5] = g; eq[i >> 5] = e; }
+    }
+    // exclusive ranks of the words' counts over the whole block, in word order; s: kSelWarps words; returns the sum over all
+    auto ranks = [&](const int (&n)[WL], int (&at)[WL], int32_t* s) {
+        int base = 0;
+#pragma unroll
+        for (int x = 0; x < WL; x++) { const int inc = warp_inclusive(n[x]); at[x] = base + inc - n[x]; base += __shfl_sync(0xffffffffu, inc, 31); }
+        const int bef = warps_before(s, base);
+#pragma unroll
+        for (int x = 0; x < WL; x++) at[x] += bef;
+        return (int)__reduce_add_sync(0xffffffffu, lane < kSelWarps ? s[lane] : 0);
+    };
+    uint32_t kept[WL]; int n[WL], at[WL];
+#pragma unroll
+    for (int x = 0; x < WL; x++) { kept[x] = gt[x] | eq[x]; n[x] = __popc(eq[x]); }
+    if (reach != keep) {   // reach - keep of the keys equal to prefix are too many: the highest slots go
+        const int all = ranks(n, at, s_d);
+#pragma unroll
+        for (int x = 0; x < WL; x++) {
+            uint32_t stay = 0, rest = eq[x];
+            for (int m = min(all - (reach - keep) - at[x], 32); m > 0 && rest; m--) { stay |= rest & (0u - rest); rest &= rest - 1; }
+            kept[x] = gt[x] | stay;
+        }
+    }
+    uint32_t hole[WL], mover[WL]; int h_at[WL];
+#pragma unroll
+    for (int x = 0; x < WL; x++) {
+        const int i = lane + 32 * x, jw = (w * ITEMS + i) * 32; const uint32_t below = i >= ITEMS ? 0u : jw + 32 <= keep ? 0xffffffffu : jw >= keep ? 0u : (1u << (keep - jw)) - 1;   // slots of the word below `keep`
+        hole[x] = ~kept[x] & below; mover[x] = kept[x] & ~below;
+    }
+#pragma unroll
+    for (int x = 0; x < WL; x++) n[x] = __popc(hole[x]);
+    ranks(n, h_at, s_c);
+#pragma unroll
+    for (int x = 0; x < WL; x++) n[x] = __popc(mover[x]);
+    ranks(n, at, s_b);
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+        const uint32_t mv = __shfl_sync(0xffffffffu, mover[i >> 5], i & 31); const int m_at = __shfl_sync(0xffffffffu, at[i >> 5], i & 31);
+        if ((mv >> lane) & 1u) list[m_at + __popc(mv & ((1u << lane) - 1))] = (uint16_t)(j0 + 32 * i);
     }
     __syncthreads();
-    block_exclusive_scan(pre_m, words, s_warp);
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+        const uint32_t hl = __shfl_sync(0xffffffffu, hole[i >> 5], i & 31); const int a_h = __shfl_sync(0xffffffffu, h_at[i >> 5], i & 31), j = j0 + 32 * i;
+        if (j < keep) src[j] = ((hl >> lane) & 1u) ? (int)list[a_h + __popc(hl & ((1u << lane) - 1))] : j;
+    }
+}
+
+// grid (8 * kv heads, sequences, layers), clusters of 8 CTAs; CTA `rank` of a cluster has words [rank * wpc, (rank + 1) * wpc) of 32 slots, warp w of it words w, w + 16, ... ITEMS: keys per thread, at most
+// as many words per warp (0: the keys are not kept). Dynamic shared memory: three words per word of slots, then the list of the CTA's free slots (16 bits each)
+template <int ITEMS>
+__global__ void __launch_bounds__(kSelThreads) paged_select_cluster_kernel(const __grid_constant__ PagedBatch b, const __grid_constant__ EvictArgs a, const int wpc) {
+    namespace cg = cooperative_groups; constexpr int CS = kSelCluster;
+    extern __shared__ __align__(16) uint32_t dyn[];
+    uint32_t* kept = dyn; int32_t* pre_h = reinterpret_cast<int32_t*>(dyn + wpc); int32_t* pre_m = pre_h + wpc; uint16_t* list = reinterpret_cast<uint16_t*>(dyn + 3 * wpc);
+    __shared__ __align__(16) int32_t hist[4][1024]; __shared__ uint32_t own[kOwn], near[kNear], sample[kSample], s_bound[2]; __shared__ int32_t s_cand[CS], s_above[CS], s_eq[CS], s_holes[CS], s_movers[CS], s_sum[3], s_warp[kSelWarps]; __shared__ int s_bin, s_left, s_n[2];
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rank = blockIdx.x % CS, kvh = blockIdx.x / CS, bi = blockIdx.y, l = blockIdx.z, S = b.slot[bi], keep = a.keep, newest = b.age[bi] - a.recent;   // ages from `newest` on are protected
+    auto peer = [&](auto* p, int r) { return cg::this_cluster().map_shared_rank(p, r); };
+    auto sync_all = [&]() { cg::this_cluster().sync(); };
+    if (tid == 0) { s_n[0] = s_n[1] = 0; s_sum[0] = s_sum[1] = s_sum[2] = 0; }
+    pdl_wait(); pdl_launch_dependents();
+    int32_t* src = a.src + (((int64_t)l * a.n + bi) * a.kv_heads + kvh) * keep;
+    if (S <= keep) { for (int j = rank * kSelThreads + tid; j < keep; j += CS * kSelThreads) src[j] = j < S ? j : -1; return; }   // (the whole cluster)
+    const int32_t* table = a.tables + (int64_t)b.seq[bi] * a.width; const float* weight = a.weight + (int64_t)(a.layer0 + l) * a.plane_stride; const int32_t* age = a.age + (int64_t)(a.layer0 + l) * a.plane_stride;
+    const int j0 = rank * wpc * 32, mine = min(max(S - j0, 0), wpc * 32), words = (mine + 31) >> 5;   // slots j0 .. j0 + mine - 1 are this CTA's; item i of a thread: j0 + tid + 512 * i
+    constexpr bool REGS = ITEMS > 0;
+    uint32_t key[REGS ? ITEMS : 1];
+    if (REGS) evict_keys(a, table, weight, age, kvh, S, newest, [&](int i) { return tid + i * kSelThreads < mine ? j0 + tid + i * kSelThreads : S; }, key);
+    auto each = [&](auto f) {   // f(key, position among the CTA's slots), a warp's lanes together; key 0 behind the last
+        if constexpr (REGS) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; i++) f(key[i], tid + i * kSelThreads);
+        } else for (int q0 = w * 32; q0 < mine; q0 += kSelThreads) f(q0 + lane < mine ? evict_key(a, table, weight, age, kvh, j0 + q0 + lane, newest) : 0u, q0 + lane);
+    };
+    __syncthreads();
+    int turn = 0;
+    auto total = [&](int v) {   // over the block; three words taken in turn: one barrier per sum
+        v = (int)__reduce_add_sync(0xffffffffu, v);
+        if (lane == 0) atomicAdd(&s_sum[turn], v);
+        __syncthreads();
+        const int t = s_sum[turn]; turn = turn == 2 ? 0 : turn + 1;
+        if (tid == 0) s_sum[turn == 2 ? 0 : turn + 1] = 0;   // read by everybody before this barrier, used after the next
+        return t;
+    };
+    auto slot_for = [&](int n, int which) {   // where a thread's n values go in a list counted by s_n[which]
+        const int inc = warp_inclusive(n); int at = 0;
+        if (lane == 31 && inc) at = atomicAdd(&s_n[which], inc);
+        return __shfl_sync(0xffffffffu, at, 31) + inc - n;
+    };
+    uint32_t prefix = 0; int left = keep;   // left: how many of the keys equal to prefix (of the keys that match it, on the way) are kept
+    bool found = false;
+    if constexpr (REGS) {   // ---- the keep-th largest key by bounds
+        auto bounds = [&](int target, int n, uint32_t& hi, uint32_t& lo) {   // where the target-th largest of n keys hardly lies above (hi) or below (lo), from the sample
+            if (w < 2) {   // warp 0 finds hi, warp 1 lo
+                uint32_t k[kSample / 32]; int n_s = 0;
+#pragma unroll
+                for (int i = 0; i < kSample / 32; i++) { k[i] = sample[i * 32 + lane]; n_s += k[i] != 0u; }
+                n_s = __reduce_add_sync(0xffffffffu, n_s);
+                const float f = (float)target / (float)n, mid = f * n_s, dev = 3.0f * sqrtf(n_s * f * (1.0f - f)) + 3.0f; const int t = w == 0 ? (int)(mid - dev) : (int)(mid + dev) + 1;   // rank in the sample
+                const uint32_t v = t < 1 ? 0xffffffffu : t > n_s ? 1u : warp_search(k, t, 1u, 0xffffffffu);
+                if (lane == 0) s_bound[w] = max(v, 1u);
+            }
+            __syncthreads();
+            hi = s_bound[0]; lo = min(s_bound[1], hi);
+        };
+        constexpr int step = kSelThreads * CS / kSample;
+        if (tid % step == 0) {   // every CTA's share of the sample, to every CTA
+            uint32_t k = 0;
+#pragma unroll
+            for (int i = 0; i < ITEMS; i++) if (tid / step % ITEMS == i) k = key[i];
+            for (int r = 0; r < CS; r++) peer(&sample[0], r)[rank * (kSample / CS) + tid / step] = k;
+        }
+        sync_all();
+        uint32_t hi, lo; int up = 0, c = 0;
+        bounds(keep, S, hi, lo);
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) { up += key[i] > hi; c += key[i] >= lo && key[i] <= hi; }
+        int at = slot_for(c, 0);
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) if (key[i] >= lo && key[i] <= hi) { if (at < kOwn) own[at] = key[i]; at++; }
+        up = total(up);
+        if (tid < CS) { peer(&s_cand[0], tid)[rank] = s_n[0]; peer(&s_above[0], tid)[rank] = up; }
+        sync_all();
+        int above = 0, between = 0, most = 0;
+#pragma unroll
+        for (int r = 0; r < CS; r++) { above += s_above[r]; between += s_cand[r]; most = max(most, s_cand[r]); }
+        int need = keep - above;   // the need-th largest of the keys between
+        found = most <= kOwn && between <= kGather * kSelThreads && need > 0 && need <= between;   // the same in every CTA of the cluster, as all that follows from it
+        if (found) {
+            auto cand = [&](int i) {   // key i of those between, whichever CTA found it
+                int r = 0;
+                while (r < CS - 1 && i >= s_cand[r]) i -= s_cand[r++];
+                return peer(&own[0], r)[i];
+            };
+            uint32_t k[kGather];
+#pragma unroll
+            for (int i = 0; i < kGather; i++) k[i] = tid + i * kSelThreads < between ? cand(tid + i * kSelThreads) : 0u;
+            if (between > kNear) {   // once more
+                sample[tid] = cand((int)((int64_t)tid * between / kSample));
+                __syncthreads();
+                bounds(need, between, hi, lo);
+            }
+            int u = 0, n = 0;
+#pragma unroll
+            for (int i = 0; i < kGather; i++) { u += k[i] > hi; n += k[i] >= lo && k[i] <= hi; }
+            int to = slot_for(n, 1);
+#pragma unroll
+            for (int i = 0; i < kGather; i++) if (k[i] >= lo && k[i] <= hi) { if (to < kNear) near[to] = k[i]; to++; }
+            u = total(u);
+            const int m = s_n[1];
+            need -= u; found = m <= kNear && need > 0 && need <= m;
+            if (found && w == 0) {
+                auto last = [&](auto size) {   // over 32 * N keys
+                    constexpr int N = decltype(size)::value;
+                    uint32_t x[N], least = 0xffffffffu; int g = 0;
+#pragma unroll
+                    for (int i = 0; i < N; i++) x[i] = i * 32 + lane < m ? near[i * 32 + lane] : 0u;
+                    const uint32_t v = warp_search(x, need, lo, hi);
+#pragma unroll
+                    for (int i = 0; i < N; i++) if (x[i] >= v && x[i] != 0u) least = min(least, x[i]);   // the smallest key that reaches it: the threshold
+                    least = __reduce_min_sync(0xffffffffu, least);
+#pragma unroll
+                    for (int i = 0; i < N; i++) g += x[i] > least;
+                    g = __reduce_add_sync(0xffffffffu, g);
+                    if (lane == 0) { s_bin = (int)least; s_left = need - g; }
+                };
+                if (m <= 256) last(std::integral_constant<int, 8>()); else if (m <= 512) last(std::integral_constant<int, 16>()); else last(std::integral_constant<int, kNear / 32>());
+            }
+            __syncthreads();
+            if (found) { prefix = (uint32_t)s_bin; left = s_left; }
+        }
+    }
+    if (!found) {   // ---- or by a radix select: digits of 8 bits, four histograms of 256 bins each, picked by lane (fewer lanes meet)
+        for (int i = tid; i < 4 * 1024; i += kSelThreads) (&hist[0][0])[i] = 0;
+        __syncthreads();
+        uint32_t mask = 0;
+#pragma unroll 1
+        for (int pass = 0; pass < 4; pass++) {
+            const int shift = 24 - 8 * pass; int32_t* hp = hist[pass];
+            each([&](uint32_t k, int) { if (k != 0u && (k & mask) == prefix) atomicAdd(&hp[((k >> shift) & 255u) * 4 + (lane & 3)], 1); });
+            sync_all();
+            int c = 0;   // thread t < 256: bin 255 - t
+            if (tid < 256) for (int r = 0; r < CS; r++) { const int4 v = *reinterpret_cast<const int4*>(peer(hp + (255 - tid) * 4, r)); c += v.x + v.y + v.z + v.w; }
+            const int inc = warp_inclusive(c), before = warps_before(s_warp, __shfl_sync(0xffffffffu, inc, 31)) + inc - c;   // keys in higher bins
+            if (tid < 256 && before < left && before + c >= left) { s_bin = 255 - tid; s_left = left - before; }
+            __syncthreads();
+            prefix |= (uint32_t)s_bin << shift; mask |= 255u << shift; left = s_left;
+            __syncthreads();
+        }
+    }
+    // ---- prefix is the keep-th largest key; of the slots that have it, the `left` lowest are kept
+    each([&](uint32_t k, int q) {
+        const uint32_t gt = __ballot_sync(0xffffffffu, k > prefix), eq = __ballot_sync(0xffffffffu, k == prefix); const int wd = q >> 5;
+        if (lane == 0 && wd < words) { kept[wd] = gt; pre_h[wd] = (int32_t)eq; }
+    });
+    __syncthreads();
+    auto ranks = [&](auto count, int32_t* pre, int32_t* sums) {   // pre[word] = sum of count over the CTA's words before it; sums[rank], in every CTA: over all of them. Thread t has words [t * per, ..)
+        const int per = (words + kSelThreads - 1) / kSelThreads, lo = min(tid * per, words), hi = min(lo + per, words);
+        int n = 0;
+        for (int wd = lo; wd < hi; wd++) n += count(wd);
+        const int inc = warp_inclusive(n); int run = warps_before(s_warp, __shfl_sync(0xffffffffu, inc, 31)) + inc - n;
+        for (int wd = lo; wd < hi; wd++) { const int c = count(wd); pre[wd] = run; run += c; }
+        if (tid == kSelThreads - 1) for (int r = 0; r < CS; r++) peer(sums, r)[rank] = run;
+        __syncthreads();   // s_warp is used again
+    };
+    ranks([&](int wd) { return __popc((uint32_t)pre_h[wd]); }, pre_m, s_eq);
+    sync_all();
+    int taken = 0;   // slots with the threshold key in the CTAs before
+    for (int r = 0; r < rank; r++) taken += s_eq[r];
+    auto below = [&](int wd) { const int j = j0 + wd * 32; return j + 32 <= keep ? 0xffffffffu : j >= keep ? 0u : (1u << (keep - j)) - 1; };   // slots of a word below `keep`
     for (int wd = tid; wd < words; wd += kSelThreads) {
         uint32_t eq = (uint32_t)pre_h[wd], take = 0;
-        for (int n = min(left - pre_m[wd], 32); n > 0 && eq; n--) { take |= eq & (0u - eq); eq &= eq - 1; }
-        const uint32_t kp = kept[wd] | take; kept[wd] = kp;
-        const int j0 = wd * 32; const uint32_t below = j0 + 32 <= keep ? 0xffffffffu : j0 >= keep ? 0u : (1u << (keep - j0)) - 1;   // slots of this word below `keep`
-        pre_h[wd] = __popc(~kp & below); pre_m[wd] = __popc(kp & ~below);
+        for (int n = min(left - taken - pre_m[wd], 32); n > 0 && eq; n--) { take |= eq & (0u - eq); eq &= eq - 1; }
+        kept[wd] |= take;
     }
     __syncthreads();
-    block_exclusive_scan(pre_h, words, s_warp);
-    block_exclusive_scan(pre_m, words, s_warp);
-    for (int j = tid; j < keep; j += kSelThreads) {
-        const int wd = j >> 5; const uint32_t bit = 1u << (j & 31), kp = kept[wd];
-        int from = j;
-        if (!(kp & bit)) {
-            const int r = pre_h[wd] + __popc(~kp & (bit - 1));   // its rank among the free slots: the mover of that rank comes here
-            int lo = keep >> 5, hi = words - 1;                  // the last word whose movers start at or before rank r
-            while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (pre_m[mid] <= r) lo = mid; else hi = mid - 1; }
-            uint32_t mv = kept[lo] & (lo * 32 >= keep ? 0xffffffffu : ~((1u << (keep - lo * 32)) - 1));
-            for (int n = r - pre_m[lo]; n > 0; n--) mv &= mv - 1;
-            from = lo * 32 + __ffs(mv) - 1;
-        }
-        src[j] = from;
+    ranks([&](int wd) { return __popc(~kept[wd] & below(wd)); }, pre_h, s_holes);
+    ranks([&](int wd) { return __popc(kept[wd] & ~below(wd)); }, pre_m, s_movers);
+    // ---- slots that stay; free slots into the list, by rank
+    for (int q = tid; j0 + q < keep && q < mine; q += kSelThreads) {
+        const int wd = q >> 5; const uint32_t bit = 1u << (q & 31), kp = kept[wd];
+        if (kp & bit) src[j0 + q] = j0 + q; else list[pre_h[wd] + __popc(~kp & (bit - 1))] = (uint16_t)q;
     }
+    sync_all();
+    // ---- movers: the free slot of the same rank, wherever in the cluster it lies
+    int rk0 = 0;
+    for (int r = 0; r < rank; r++) rk0 += s_movers[r];
+    for (int q = max(keep - j0, 0) + tid; q < mine; q += kSelThreads) {
+        const int wd = q >> 5; const uint32_t bit = 1u << (q & 31);
+        if (!(kept[wd] & bit)) continue;
+        int rk = rk0 + pre_m[wd] + __popc(kept[wd] & ~below(wd) & (bit - 1)), r = 0;
+        while (r < CS - 1 && rk >= s_holes[r]) rk -= s_holes[r++];
+        src[r * wpc * 32 + peer(list, r)[rk]] = j0 + q;
+    }
+    sync_all();   // nobody leaves while its shared memory may still be read
 }
 
 // grid (ceil(keep / 256), kv heads * sequences, layers) x 256 threads: a warp per 32 destinations. CH: 16-byte chunks of a head row
@@ -169,14 +400,33 @@ __global__ void __launch_bounds__(256) paged_move_kernel(const __grid_constant__
 
 }  // namespace
 
-cudaError_t configure_paged_evict(const PagedCtx&) { return cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSmemMax - kBins * 4 - 1024); }
+cudaError_t configure_paged_evict(const PagedCtx&) {   // shared-memory opt-in, per device
+    const cudaError_t e = cudaFuncSetAttribute(paged_select_cluster_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, KATA_PAGED_MAX_SLOTS / 32 / kSelCluster * 76);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(paged_select_cluster_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kCluMax / 32 / kSelCluster * 76);
+}
 
 cudaError_t launch_paged_evict(PagedCtx& c, int layer, int n_layers, const PagedBatch& b, int keep, int sink, int recent, int32_t* src, cudaStream_t s) {
     EvictArgs a{}; a.keep = keep; a.sink = sink; a.recent = recent; a.width = c.width; a.page_shift = c.page_shift; a.kv_heads = c.cfg.kv_heads; a.n = b.n; a.layer0 = layer;
     a.plane_stride = c.rows_per_layer * c.cfg.kv_heads; a.tables = c.d_table; a.weight = (float*)c.plane[KATA_PAGED_WEIGHT]; a.age = (int32_t*)c.plane[KATA_PAGED_AGE]; a.src = src;
     int most = 0; for (int i = 0; i < b.n; i++) most = std::max(most, b.slot[i]);
-    const int words = (most + 31) / 32, budget = kSelSmemMax - kBins * 4 - 1024, cached = words * 12 + words * 128 <= budget ? 1 : 0;   // keys of up to some 48,000 slots are kept in shared memory, else read again in every pass
-    cudaError_t e = launch_pdl(paged_select_kernel, dim3(c.cfg.kv_heads, b.n, n_layers), dim3(kSelThreads), (size_t)words * (cached ? 140 : 12), s, b, a, words, cached);
+    cudaError_t e;
+    const int64_t segments = (int64_t)c.cfg.kv_heads * b.n * n_layers;
+    if (most <= kSelOne || (most <= kCluMax && segments >= kSelMany)) {
+        const dim3 grid(c.cfg.kv_heads, b.n, n_layers);
+#define KATA_SELECT(N) launch_pdl(paged_select_kernel<N>, grid, dim3(kSelThreads), 0, s, b, a)
+        const int items = (most + kSelThreads - 1) / kSelThreads;
+        static_assert(kCluMax == 64 * kSelThreads, "the largest variant holds what a cluster holds");
+        e = items <= 2 ? KATA_SELECT(2) : items <= 10 ? KATA_SELECT(10) : items <= 24 ? KATA_SELECT(24) : KATA_SELECT(64);
+#undef KATA_SELECT
+    } else {
+        const int wpc = ((most + 31) / 32 + kSelCluster - 1) / kSelCluster;
+        static_assert(KATA_PAGED_MAX_SLOTS / kSelCluster <= 65536 && kCluSlots % (32 * kSelCluster) == 0, "free slots are listed with 16 bits");
+        cudaLaunchConfig_t cfg{}; cfg.gridDim = dim3(kSelCluster * c.cfg.kv_heads, b.n, n_layers); cfg.blockDim = dim3(kSelThreads); cfg.dynamicSmemBytes = (size_t)wpc * 76; cfg.stream = s;
+        cudaLaunchAttribute at[2]; at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization; at[0].val.programmaticStreamSerializationAllowed = 1;
+        at[1].id = cudaLaunchAttributeClusterDimension; at[1].val.clusterDim.x = kSelCluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+        cfg.attrs = at; cfg.numAttrs = 2;
+        e = most <= kCluMax ? cudaLaunchKernelEx(&cfg, paged_select_cluster_kernel<8>, b, a, wpc) : most <= 4 * kCluMax ? cudaLaunchKernelEx(&cfg, paged_select_cluster_kernel<32>, b, a, wpc) : cudaLaunchKernelEx(&cfg, paged_select_cluster_kernel<0>, b, a, wpc);
+    }
     if (e != cudaSuccess) return e;
     c.launches++;
     if (most <= keep) return cudaGetLastError();   // nothing to move in any sequence

@@ -37,7 +37,7 @@ def _context(capi, slots, layout=(24, 4, 256), page=16, kv="fp16", fill=None, sp
     """A context whose sequences hold `slots` reserved slots, pages interleaved between them (16 slots at a time, round robin)."""
     H, KH, D = layout
     top = max(max(slots), 1)
-    ctx = capi.PagedContext(n_layers, len(slots), sum(-(-s // page) for s in slots) + spare, page, top + 2 * page, heads=H, kv_heads=KH, head_dim=D, kv_mode=kv, rot_dim=kw.pop("rot_dim", 64), **kw)
+    ctx = capi.PagedContext(n_layers, len(slots), sum(-(-s // page) for s in slots) + spare, page, min(top + 2 * page, 524288), heads=H, kv_heads=KH, head_dim=D, kv_mode=kv, rot_dim=kw.pop("rot_dim", 64), **kw)
     step = max(16, top // 8)
     for upto in range(step, top + step, step):
         for s, n in enumerate(slots):
@@ -327,6 +327,43 @@ def test_eviction_of_several_layers_and_of_long_sequences(capi):
             assert torch.equal(got[stay], torch.arange(keep, device="cuda").expand(2, keep)[stay])
             assert all((got[h][~stay[h]].diff() > 0).all() for h in range(2))
             assert torch.equal(_kv(ctx, l, s, keep)[0].permute(1, 0, 2), k[got, torch.arange(2, device="cuda")[:, None]])
+    ctx.close()
+
+
+def _expected_on_gpu(w, keep):
+    """[kv_heads][n] weights -> src [kv_heads][keep], nothing protected."""
+    order = torch.sort(w, dim=-1, descending=True, stable=True).indices[:, :keep]
+    kept = torch.zeros_like(w, dtype=torch.bool).scatter_(-1, order, True)
+    src = torch.arange(keep, device=w.device).repeat(w.shape[0], 1)
+    for h in range(w.shape[0]):
+        src[h, ~kept[h, :keep]] = torch.nonzero(kept[h, keep:])[:, 0] + keep
+    return src
+
+
+@pytest.mark.parametrize("values", ["spread", "eighths", "equal", "sparse", "rising", "falling"])
+@pytest.mark.parametrize("n,slots", [(1, 5120), (1, 5121), (2, 9999), (64, 1500), (40, 5300), (33, 12289), (1, 32768), (1, 32769), (1, 131072), (1, 131073), (1, 524288)])
+def test_selection_of_any_size_and_any_ties(capi, n, slots, values):
+    """One CTA or a cluster per head, bounds or a radix select, few and many heads: the same slots."""
+    if n * slots > 100000 and values in ("rising", "sparse"):
+        values = "spread"
+    g = _gen(slots + n)
+    ctx = _context(capi, [slots] * n, (2, 2, 128), 1024 if slots > 20000 else 64, weights=True, spare=0)
+    mk = {"spread": lambda *s: torch.rand(s, generator=g, device="cuda").square(), "eighths": lambda *s: (torch.rand(s, generator=g, device="cuda") * 8).floor(), "equal": lambda *s: torch.zeros(s, device="cuda"),
+          "sparse": lambda *s: torch.rand(s, generator=g, device="cuda") * (torch.rand(s, generator=g, device="cuda") < 0.1), "rising": lambda *s: torch.arange(s[-1], device="cuda").expand(s).float(),
+          "falling": lambda *s: -torch.arange(s[-1], device="cuda").expand(s).float()}[values]
+    w = mk(n, 2, slots)
+    ctx.plane(0, "age").fill_(10 ** 6)
+    page = ctx.page_size
+    rows = torch.stack([_rows(ctx, s, slots) for s in range(n)])
+    for keep in (1, slots // 8, slots // 2, slots - 1):
+        for s in range(n):
+            ctx.plane(0, "weight")[rows[s] // page, :, rows[s] % page] = w[s].T
+        src = ctx.evict(0, range(n), [slots] * n, keep, 10 ** 7)
+        ctx.check()
+        for s in range(n):
+            assert torch.equal(src[s].long(), _expected_on_gpu(w[s], keep)), (keep, s)
+        assert torch.equal(torch.stack([_per_head(ctx, 0, "weight", s, keep) for s in range(n)]), w.gather(2, src.long()))
+        ctx.plane(0, "age").fill_(10 ** 6)
     ctx.close()
 
 
