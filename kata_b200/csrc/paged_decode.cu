@@ -5,22 +5,23 @@
 // Bound by HBM (4096 bytes of K+V per slot at fp16 with 4 heads of 256, each read once), so the work split is that of the contiguous decode kernel:
 // the tiles (16 or 32 slots of one KV head, 16 KiB of K+V) of all (sequence, KV head) segments form one list, cut into one contiguous range per SM, the
 // ranges' partial rows joined by the last CTA of a segment (at most 8 of them) or by a combine grid. Inside a CTA four rings of a score warp and two value warps take
-// the tiles in turn; producer warps refill the
-// rings' stages with TMA. What pages change:
+// the tiles in turn; producer warps refill the rings' stages with TMA. The three kinds of warps pass from one segment into the next on their own (mbarriers for what they hand over, named barriers
+// within a kind): the producers and the score warps work on the next segment while the value warps add the rings up and write the rows. With all of them stopping at a segment's end, 32 int8
+// sequences of 300 to 32K slots took 202 us (182 now), 256 fp16 sequences of 200 slots 68 us (62). What pages change:
 //  - A tile is made of 16-slot groups, and a group never crosses a page (pages are powers of two from 16 slots on). The tensor map is a rank-5 view of
 //    the pool, {128-byte column block, 16 rows, column blocks, 16-row groups, KV heads}: the group is a coordinate, so one instruction
 //    brings the 16 or 32 slots of a tile wherever their page lies, in the same shared-memory order ([group][column block][16 rows][128 bytes], swizzled) for
 //    every page size. Pages of 16 slots under 32-slot tiles take two instructions.
 //  - The producer reads the page number of a tile three tiles before it needs it. In the int8 mode a ring has a producer warp
-//    of its own, whose lanes fetch the slots' K and V scales as well, three tiles ahead, and leave them in shared memory: with the loads in the score warp it waited for them (359 us for 32 sequences of 300 to
-//    32K slots), and so it did with one warp for the four rings' scales (352 us).
+//    of its own, whose lanes fetch the slots' K and V scales as well, three tiles ahead, and leave them in shared memory: the score warp waited when it had the loads (359 us for 32 sequences of 300 to
+//    32K slots, 228 with a producer per ring, all else as it was then), and so it did with one warp for the four rings' scales (352 us).
 //  - Groups behind the last slot repeat the last page (their table entry may not exist); such slots are masked, and their V rows zeroed in shared
 //    memory, so whatever lies there (NaN included) has no part in the result.
 // Head layouts: head_dim 256 or 128, up to 16 query heads per KV head; tokens beyond 16 / group run as further passes.
 //
 // The matrix instructions take the keys (and the head dims of V) as their 16 rows and the query rows as their 8 columns: S^T = K Q^T, O^T = V^T P^T. One token of up to 8 heads
 // per KV head then costs half the instructions, softmax and registers of a 16-row block (NR = 1 against NR = 2 column tiles); the query's fragments stay in registers
-// for the whole segment. With the query rows as the 16 rows instead, 32 sequences of 300 to 32K int8 slots took 280 us.
+// for the whole segment. With the query rows as the 16 rows instead, 32 sequences of 300 to 32K int8 slots took 280 us (228 at that time).
 //
 // Precision: fp16 products, fp32 sums. The exponent carries an offset (kPShift) so that p lies high in fp16's range: it cancels in p / l and keeps
 // small p out of the subnormals. p goes into P.V in two fp16 terms (about 22 bits; int8 caches with 16-bit outputs: one term, 2^-11 relative, there the second costs time), int8 codes are taken
@@ -38,44 +39,48 @@ using namespace ptx;
 
 constexpr int kRings = 4, kMaxStages = 6;
 
-// The barrier block: per ring and stage 'full' and 'empty', then per ring two 'P full' and two 'P empty'.
-constexpr int kOffEBars = kRings * kMaxStages * 8, kOffPBars = 2 * kOffEBars, kBarBytes = kOffPBars + kRings * 32;
+// The barrier block: per ring and stage 'full' and 'empty', per ring two 'P full' and two 'P empty', then two 'sums full' and two 'sums empty'.
+constexpr int kOffEBars = kRings * kMaxStages * 8, kOffPBars = 2 * kOffEBars, kOffSBars = kOffPBars + kRings * 32, kBarBytes = kOffSBars + 128;
 
-template <int HD, bool K8> struct PGeo {
-    static constexpr int kThreads = (3 * kRings + (K8 ? kRings : 1)) * 32;               // fp16: one producer warp, lane r for ring r (in step: 142 us for eight sequences of 16K to 32K slots, 154 with one per ring); int8: one per ring
+template <int HD, bool K8, int NR> struct PGeo {   // NR: column tiles of 8 query rows
+    static constexpr int kThreads = (3 * kRings + (K8 ? kRings : 1)) * 32;               // fp16: one producer warp, lane r for ring r (in step: 121 us for 37 sequences of 5,200 slots, 127 with one per ring, 140 with one whose lanes drift apart); int8: one per ring
     static constexpr int kRowBytes = HD * (K8 ? 1 : 2);                                  // bytes of a head row
     static constexpr int kNK = (HD == 256 && !K8) ? 1 : 2, kTile = 16 * kNK;             // 16-slot groups and slots per tile
     static constexpr int kGroupBytes = 16 * kRowBytes, kHalfBytes = kNK * kGroupBytes;   // K (or V) of one group, of one tile
     static constexpr int kStageBytes = 2 * kHalfBytes, kStages = kStageBytes == 16384 ? 3 : 6;
-    static constexpr int kMergeStride = HD + 8;                                          // floats per row of the cross-ring merge buffer
     static constexpr int kRingBytes = kStages * kStageBytes;
-    static constexpr int kQStride = HD * 2 + 16, kQBytes = 16 * kQStride;                // the query block: fp16 rows, 16 bytes of padding
-    static constexpr int kPStride = 32 * kNK + 16, kPTerm = 16 * kPStride, kPBytes = 2 * kPTerm + 64;   // a P slot: two fp16 blocks (heads and remainders), 16 rescale factors
+    static constexpr int kQStride = HD * 2 + 16, kQBytes = NR * 8 * kQStride;                // the query block: fp16 rows, 16 bytes of padding
+    static constexpr int kPStride = 32 * kNK + 16, kPTerm = NR * 8 * kPStride, kPBytes = 2 * kPTerm + 64;   // a P slot: two fp16 blocks (heads and remainders), 16 rescale factors
     static constexpr int kPShift = K8 ? 5 : 15;                                          // p is carried as 2^kPShift * p (int8: p times a scale up to 516 has to stay below 65504)
-    static constexpr int kOffBars = kQBytes, kOffMl = kOffBars + kBarBytes, kOffPair = kOffMl + 512, kOffScale = kOffPair + kRings * 2 * kPBytes, kOffStages = kOffScale + (K8 ? kRings * kStages * 128 : 0);   // scales: [ring][stage][32 slots] K and V packed
+    static constexpr int kAcc = HD / 32 * NR * 4, kRedBytes = 2 * kAcc * 128;            // accumulators per value-warp lane; the block in which the rings add them up
+    // NR = 1: a block of its own, and two slots for the rings' (m, l): the score warps go on into the next segment. NR = 2: no room, it lies where the P slots are and the score warps wait.
+    static constexpr int kSums = NR == 1 ? 2 : 1;
+    static constexpr int kOffBars = kQBytes, kOffMl = kOffBars + kBarBytes, kOffPair = kOffMl + kSums * 512 + 128, kOffRed = kOffPair + (NR == 1 ? kRings * 2 * kPBytes : 0);
+    static constexpr int kOffScale = NR == 1 ? kOffRed + kRedBytes : kOffPair + (kRings * 2 * kPBytes > kRedBytes ? kRings * 2 * kPBytes : kRedBytes), kOffStages = kOffScale + (K8 ? kRings * kStages * 128 : 0);   // scales: [ring][stage][32 slots] K and V packed
     static constexpr int kSmem = kOffStages + 1024 + kRings * kRingBytes;
-    static_assert(16 * kMergeStride * 4 <= kRingBytes && kSmem <= 232448, "shared memory");
+    static_assert(kSmem <= 232448, "shared memory");
 };
+constexpr int kMaxCtas = 192;
 struct PagedPlan {
     int32_t two_terms;                                              // P in two fp16 terms (fp32 outputs; always where it is free)
-    int32_t n, T, group, kv_heads, n_ctas, q_tiles, r_tiles, cps;   // as in the contiguous kernel: CTA c owns tiles [c*q + min(c,r), ..), or (cps > 0) a share of one segment
+    int32_t n, T, group, kv_heads, n_ctas;
     int32_t tok_stride, tok0, page_shift, width, groups_per_box, merge_in_kernel;
     int64_t layer_row0;
+    int32_t cut[kMaxCtas + 1];                     // CTA c has the tiles [cut[c], cut[c + 1])
     int32_t seq[KATA_PAGED_MAX_BATCH];
     int32_t kend[KATA_PAGED_MAX_BATCH];            // slots the last token of this pass sees (may be 0)
-    int32_t tile_start[KATA_PAGED_MAX_BATCH + 1];
+    int32_t tile_start[KATA_PAGED_MAX_BATCH + 1];  // first tile of a sequence; its tiles are those of KV head 0, of head 1, ...
 };
-static_assert(sizeof(PagedPlan) + 2 * sizeof(CUtensorMap) + 128 <= 4096, "kernel parameters");
+static_assert(sizeof(PagedPlan) + 2 * sizeof(CUtensorMap) + 128 <= 32764, "kernel parameters");
 
 __host__ __device__ __forceinline__ int plan_ntiles(const PagedPlan& p, int b) { return (p.tile_start[b + 1] - p.tile_start[b]) / p.kv_heads; }
-__host__ __device__ __forceinline__ int plan_first_tile(const PagedPlan& p, int c) {
-    if (p.cps) { const int seg = c / p.cps, j = c - seg * p.cps, nt = plan_ntiles(p, 0); return seg * nt + (int)((int64_t)nt * j / p.cps); }
-    return c * p.q_tiles + (c < p.r_tiles ? c : p.r_tiles);
-}
-__host__ __device__ __forceinline__ int plan_cta_of_tile(const PagedPlan& p, int tile) {
-    if (p.cps) { const int nt = plan_ntiles(p, 0), seg = tile / nt, lt = tile - seg * nt; return seg * p.cps + (int)(((int64_t)(lt + 1) * p.cps + nt - 1) / nt) - 1; }
-    const int big = p.r_tiles * (p.q_tiles + 1);
-    return tile < big ? tile / (p.q_tiles + 1) : p.r_tiles + (tile - big) / p.q_tiles;
+// The first and the last CTA of a segment, from CTA c that has some of it.
+__host__ __device__ __forceinline__ int plan_first_cta(const PagedPlan& p, int c, int seg_first) { while (p.cut[c] > seg_first) c--; return c; }
+__host__ __device__ __forceinline__ int plan_last_cta(const PagedPlan& p, int c, int seg_end) { while (p.cut[c + 1] < seg_end) c++; return c; }
+__host__ __device__ __forceinline__ int plan_cta_of(const PagedPlan& p, int tile) {   // the CTA that has a tile
+    int lo = 0, hi = p.n_ctas - 1;
+    while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (p.cut[mid] <= tile) lo = mid; else hi = mid - 1; }
+    return lo;
 }
 
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const void* tmap, int x, int r, int c, int g, int h, uint32_t bar) {
@@ -101,8 +106,8 @@ __device__ __forceinline__ void q_frags(const uint32_t q_sm, const int stride, c
 
 // Score warp, one tile: s[sb][nr] = the fragment of 16-slot group sb and column tile nr, scaled (int8). qf: the query's fragments (NR = 1).
 template <int HD, bool K8, int NR>
-__device__ __forceinline__ void paged_scores(const uint32_t q_sm, const uint32_t k_sm, const uint32_t (&qf)[HD / 16][2], const float (&ks)[PGeo<HD, K8>::kNK][2], const int lane, float (&s)[PGeo<HD, K8>::kNK][NR][4]) {
-    using G = PGeo<HD, K8>; constexpr int NK = G::kNK;
+__device__ __forceinline__ void paged_scores(const uint32_t q_sm, const uint32_t k_sm, const uint32_t (&qf)[HD / 16][2], const float (&ks)[PGeo<HD, K8, NR>::kNK][2], const int lane, float (&s)[PGeo<HD, K8, NR>::kNK][NR][4]) {
+    using G = PGeo<HD, K8, NR>; constexpr int NK = G::kNK;
     const uint32_t rx = lane & 7, hi = lane >> 4, ka = k_sm + (rx + ((lane >> 3) & 1) * 8) * 128;   // lanes 0-15: slots 0-15 at one chunk, lanes 16-31: at the next
     const uint32_t ko[4] = {((0 + hi) ^ rx) << 4, ((2 + hi) ^ rx) << 4, ((4 + hi) ^ rx) << 4, ((6 + hi) ^ rx) << 4};
     float s2[NK][NR][4];   // a second accumulator chain
@@ -172,8 +177,8 @@ __device__ __forceinline__ void paged_softmax(float (&s)[NK][NR][4], RowsState<N
 
 // P goes to shared memory as [query row][slot] fp16, heads and (two terms) remainders; the rescale factors behind it.
 template <int HD, bool K8, int NR>
-__device__ __forceinline__ void paged_publish(const uint32_t p_sm, float* alpha, const float (&pr)[PGeo<HD, K8>::kNK][NR][4], const float (&al)[NR][2], const int two_terms, const int lane) {
-    using G = PGeo<HD, K8>; constexpr int NK = G::kNK;
+__device__ __forceinline__ void paged_publish(const uint32_t p_sm, float* alpha, const float (&pr)[PGeo<HD, K8, NR>::kNK][NR][4], const float (&al)[NR][2], const int two_terms, const int lane) {
+    using G = PGeo<HD, K8, NR>; constexpr int NK = G::kNK;
 #pragma unroll
     for (int nr = 0; nr < NR; nr++) {
         uint32_t hi[2 * NK], lo[2 * NK];   // 8-slot blocks
@@ -203,7 +208,7 @@ template <int HD, int NR> struct ValueAcc {
 };
 template <int HD, bool K8, int NR, bool TWO>
 __device__ __forceinline__ void paged_values(const uint32_t v_sm, const uint32_t p_sm, const float* alpha, ValueAcc<HD, NR>& st, const int lane, const int vh) {
-    using G = PGeo<HD, K8>; constexpr int NK = G::kNK;
+    using G = PGeo<HD, K8, NR>; constexpr int NK = G::kNK;
     float2 al[NR]; uint32_t ph[NR][2 * NK], pl[NR][2 * NK];
 #pragma unroll
     for (int nr = 0; nr < NR; nr++) {
@@ -263,22 +268,24 @@ __device__ __forceinline__ void paged_values(const uint32_t v_sm, const uint32_t
 
 struct PagedOut { const float* gate; void* out; int32_t kind; float* fin_ml; };   // fin_ml: joined (m, 1 / l) per (segment, row), with weights only
 
-// Final value of row r of a segment, dims d and d + 1: normalised, gated, stored. A row that saw no slot has l = 0 and gets zeros.
-template <int HD> __device__ __forceinline__ void paged_emit(const PagedPlan& p, const PagedOut& o, int b, int kvh, int r, int d, float M, float L, float A0, float A1) {
-    const int t = r / p.group, head = kvh * p.group + (r - t * p.group);
-    const int64_t oi = (((int64_t)b * p.tok_stride + p.tok0 + t) * (p.kv_heads * p.group) + head) * HD + d;
-    float y0 = A0 / L, y1 = A1 / L;
-    if (o.gate) { const float2 gt = *reinterpret_cast<const float2*>(o.gate + oi); y0 *= sigmoid_fast(gt.x); y1 *= sigmoid_fast(gt.y); }
-    if (L == 0.0f) { y0 = 0.0f; y1 = 0.0f; }
-    store_act2(o.out, oi, y0, y1, o.kind);
-    if (o.fin_ml && d == 0) *reinterpret_cast<float2*>(o.fin_ml + ((int64_t)(b * p.kv_heads + kvh) * 16 + r) * 2) = make_float2(M, 1.0f / L);
+// Final value of row r of a segment, dims d and d + 1: normalised, gated, stored. A row that saw no slot has L = 0 and gets zeros.
+template <int HD> __device__ __forceinline__ int64_t paged_out_at(const PagedPlan& p, int b, int kvh, int r, int d) {
+    const int t = r / p.group;
+    return (((int64_t)b * p.tok_stride + p.tok0 + t) * (p.kv_heads * p.group) + kvh * p.group + r - t * p.group) * HD + d;
+}
+__device__ __forceinline__ float2 paged_gate(const PagedOut& o, int64_t at) { return o.gate ? __ldg(reinterpret_cast<const float2*>(o.gate + at)) : make_float2(0.0f, 0.0f); }
+__device__ __forceinline__ void paged_emit(const PagedPlan& p, const PagedOut& o, int b, int kvh, int r, int d, int64_t at, float2 gate, float M, float L, float A0, float A1) {
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L; float2 y = make_float2(L == 0.0f ? 0.0f : A0 * inv, L == 0.0f ? 0.0f : A1 * inv);
+    if (o.gate) { y.x *= sigmoid_fast(gate.x); y.y *= sigmoid_fast(gate.y); }
+    store_act2(o.out, at, y.x, y.y, o.kind);
+    if (o.fin_ml && d == 0) *reinterpret_cast<float2*>(o.fin_ml + ((int64_t)(b * p.kv_heads + kvh) * 16 + r) * 2) = make_float2(M, 1.0f / L);   // for the weights
 }
 
 template <int HD, bool K8, int NR>   // NR: column tiles of 8 query rows
-__global__ void __launch_bounds__(PGeo<HD, K8>::kThreads, 1) paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedPlan p,
+__global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ PagedPlan p,
                                                                    const int32_t* __restrict__ tables, const __half* __restrict__ q16, const PagedOut o, const __half* __restrict__ ksc, const __half* __restrict__ vsc,
                                                                    float* scores, float* scratch_o, float* scratch_ml, int32_t* counters, int32_t* err) {
-    using G = PGeo<HD, K8>; constexpr int kStages = G::kStages, kTile = G::kTile, NK = G::kNK;
+    using G = PGeo<HD, K8, NR>; constexpr int kStages = G::kStages, kTile = G::kTile, NK = G::kNK;
     if (threadIdx.x == 0) { prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, h = w >> 2, ring = (h == 3 && !K8) ? lane & 3 : w & 3, g = lane >> 2, t4 = lane & 3;   // h = 0 score warp, 1 and 2 value warps, 3 producer
@@ -287,230 +294,312 @@ __global__ void __launch_bounds__(PGeo<HD, K8>::kThreads, 1) paged_decode_kernel
     const uint32_t stage_off = ((sm_base + G::kOffStages + 1023u) & ~1023u) - sm_base, ring_stage0 = sm_base + stage_off + ring * G::kRingBytes;
     const uint32_t pfull = sm_base + G::kOffBars + kOffPBars + ring * 16, pempty = pfull + kRings * 16;
     const int p_off = G::kOffPair + ring * 2 * G::kPBytes;
-    float* sm_ml = reinterpret_cast<float*>(smem + G::kOffMl);
+    float* sm_ml = reinterpret_cast<float*>(smem + G::kOffMl); float* joined_ml = sm_ml + G::kSums * kRings * 32; float* red = reinterpret_cast<float*>(smem + G::kOffRed);
     __shared__ int s_flag;
+    const uint32_t sfull = sm_base + G::kOffBars + kOffSBars, sempty = sfull + 16;
+    auto score_sync = []() { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    auto value_sync = []() { asm volatile("bar.sync 2, 256;" ::: "memory"); };
 
     if (h == 0 && lane == 0) { for (int s = 0; s < kStages; s++) { mbar_init(bars + s * 8, 1); mbar_init(ebars + s * 8, 3); } for (int s = 0; s < 2; s++) { mbar_init(pfull + s * 8, 1); mbar_init(pempty + s * 8, 2); } }
+    if (tid == 0) { for (int s = 0; s < G::kSums; s++) { mbar_init(sfull + s * 8, kRings); mbar_init(sempty + s * 8, 2 * kRings); } }
     fence_mbar_init();
     __syncthreads();
     pdl_wait(); pdl_launch_dependents();   // the set-up above overlapped the previous kernel's tail; nothing it wrote is read before this
 
     const int kvh_n = p.kv_heads, rows = p.group * p.T, srow = NR * 8, mask = (1 << p.page_shift) - 1;
-    int tile = plan_first_tile(p, blockIdx.x); const int tile_end = plan_first_tile(p, blockIdx.x + 1);
-    int b = 0; uint32_t it = 0; bool dead = false;   // it: tiles this ring has worked on so far
+    int tile = p.cut[blockIdx.x]; const int tile_end = p.cut[blockIdx.x + 1];
+    int b = 0; uint32_t it = 0, n_segs = 0; bool dead = false;   // it: tiles this ring has worked on so far; n_segs: segments
+    // The three kinds of warps go from segment to segment on their own; barriers in shared memory hold them together.
 
-    while (tile < tile_end) {
-        while (p.tile_start[b + 1] <= tile) b++;
-        const int nt = plan_ntiles(p, b), kvh = (tile - p.tile_start[b]) / nt, lt0 = (tile - p.tile_start[b]) - kvh * nt;
-        const int seg_first = p.tile_start[b] + kvh * nt, seg_end = seg_first + nt, my_end = min(tile_end, seg_end), n_here = my_end - tile;
-        const int kend = p.kend[b], last = max(kend - 1, 0);
-        const int32_t* table = tables + (int64_t)p.seq[b] * p.width;
-        const int n_mine = n_here > ring ? (n_here - ring + kRings - 1) / kRings : 0;   // this ring's tiles: lt0 + ring, lt0 + ring + 4, ...
-        const uint32_t it_seg = it;
-        const int all_see = kend - p.T + 1;   // slots below this are seen by every row (columns that hold no query too: nobody reads what they get)
-
-        if (h == 3) {
-            // ---- producer: brings in the ring's tiles, refilling a stage as soon as its three warps have released it; page numbers are read three tiles
-            // ahead. int8: lane j also fetches the K and V scale of slot j, three tiles ahead (under load a request takes as long as all that is in flight before it), the page number of
-            // that three tiles earlier still, and stores it before the tile's copy is issued. Unrolled by three so that every load has registers of its own.
-            int32_t pg[3][2], spg[3]; unsigned short sc8[3][2];
-            auto first_slot = [&](int i) { return (lt0 + ring + i * kRings) * kTile; };
-            auto load_pages = [&](int i, int32_t (&x)[2]) {
-                x[0] = __ldcg(table + (min(first_slot(i), last) >> p.page_shift));
-                x[1] = p.groups_per_box < NK ? __ldcg(table + (min(first_slot(i) + 16, last) >> p.page_shift)) : 0;
-            };
-            auto scale_slot = [&](int i) { return min(first_slot(i) + lane, last); };   // slots behind the last repeat it: finite scales, and probabilities 0
-            auto scale_page = [&](int i) { return __ldcg(table + (scale_slot(i) >> p.page_shift)); };
-            auto load_scales = [&](int i, int32_t page, unsigned short (&x)[2]) {
-                const int64_t at = (((int64_t)page << p.page_shift) + (scale_slot(i) & mask)) * kvh_n + kvh;   // ksc, vsc: this layer's planes
-                x[0] = __ldcg(reinterpret_cast<const unsigned short*>(ksc) + at); x[1] = __ldcg(reinterpret_cast<const unsigned short*>(vsc) + at);
-            };
-            if (issues) { load_pages(0, pg[0]); load_pages(1, pg[1]); load_pages(2, pg[2]); }
-            if (K8) {
+    if (h == 3) {
+        if (tile >= tile_end) return;
+        // ---- producer: brings in the ring's tiles, refilling a stage as soon as its three warps have released it; page numbers are read three tiles
+        // ahead. int8: lane j also fetches the K and V scale of slot j, three tiles ahead (under load a request takes as long as all that is in flight before it), the page number of
+        // that three tiles earlier still, and stores it before the tile's copy is issued. Unrolled by three so that every load has registers of its own. What the first three tiles of the next
+        // segment need is requested during this one (148 int8 sequences of 3,600 slots, four segments per CTA: 203 us without).
+        struct Seg { int kvh, lt0, n_here, n_mine, last; const int32_t* table; };
+        auto segment = [&](int first) {
+            while (p.tile_start[b + 1] <= first) b++;
+            const int nt = plan_ntiles(p, b), kvh = (first - p.tile_start[b]) / nt, lt0 = first - p.tile_start[b] - kvh * nt, n_here = min(tile_end - first, nt - lt0);
+            return Seg{kvh, lt0, n_here, n_here > ring ? (n_here - ring + kRings - 1) / kRings : 0, max(p.kend[b] - 1, 0), tables + (int64_t)p.seq[b] * p.width};
+        };
+        auto first_slot = [&](const Seg& g, int i) { return (g.lt0 + ring + i * kRings) * kTile; };
+        auto load_pages = [&](const Seg& g, int i, int32_t (&x)[2]) {
+            x[0] = __ldcg(g.table + (min(first_slot(g, i), g.last) >> p.page_shift));
+            x[1] = p.groups_per_box < NK ? __ldcg(g.table + (min(first_slot(g, i) + 16, g.last) >> p.page_shift)) : 0;
+        };
+        auto scale_slot = [&](const Seg& g, int i) { return min(first_slot(g, i) + lane, g.last); };   // slots behind the last repeat it: finite scales, and probabilities 0
+        auto scale_page = [&](const Seg& g, int i) { return __ldcg(g.table + (scale_slot(g, i) >> p.page_shift)); };
+        auto load_scales = [&](const Seg& g, int i, int32_t page, unsigned short (&x)[2]) {
+            const int64_t at = (((int64_t)page << p.page_shift) + (scale_slot(g, i) & mask)) * kvh_n + g.kvh;   // ksc, vsc: this layer's planes
+            x[0] = __ldcg(reinterpret_cast<const unsigned short*>(ksc) + at); x[1] = __ldcg(reinterpret_cast<const unsigned short*>(vsc) + at);
+        };
+        Seg sg = segment(tile), next = sg; int32_t pg[3][2], npg[3][2], spg[3], nspg[3]; unsigned short sc8[3][2], nsc8[3][2];
+        if (issues) { load_pages(sg, 0, pg[0]); load_pages(sg, 1, pg[1]); load_pages(sg, 2, pg[2]); }
+        if (K8) {
 #pragma unroll
-                for (int j = 0; j < 3; j++) spg[j] = scale_page(j);
+            for (int j = 0; j < 3; j++) spg[j] = scale_page(sg, j);
 #pragma unroll
-                for (int j = 0; j < 3; j++) { load_scales(j, spg[j], sc8[j]); spg[j] = scale_page(j + 3); }
+            for (int j = 0; j < 3; j++) { load_scales(sg, j, spg[j], sc8[j]); spg[j] = scale_page(sg, j + 3); }
+        }
+        while (true) {
+            tile += sg.n_here;
+            const bool more = tile < tile_end;
+            if (more) {
+                next = segment(tile);
+                if (issues) { load_pages(next, 0, npg[0]); load_pages(next, 1, npg[1]); load_pages(next, 2, npg[2]); }
+                if (K8) { nspg[0] = scale_page(next, 0); nspg[1] = scale_page(next, 1); nspg[2] = scale_page(next, 2); }
             }
-            for (int i0 = 0; i0 < n_mine; i0 += 3)
+            const int n_steps = K8 ? sg.n_mine : (sg.n_here + kRings - 1) / kRings;   // the same for all lanes: they stay in step
+            auto next_scales = [&]() {
+#pragma unroll
+                for (int j = 0; j < 3; j++) { load_scales(next, j, nspg[j], nsc8[j]); nspg[j] = scale_page(next, j + 3); }
+            };
+            if (K8 && more && n_steps <= 3) next_scales();
+            for (int i0 = 0; i0 < n_steps; i0 += 3) {
+                if (K8 && more && i0 == 3) next_scales();
 #pragma unroll
                 for (int j = 0; j < 3; j++) {
                     const int i = i0 + j;
-                    if (i >= n_mine) break;
+                    if (i >= n_steps) break;
+                    const bool has = issues && i < sg.n_mine;
                     const uint32_t cur = it + (uint32_t)i, sx = cur % kStages, bar = bars + sx * 8, dst = ring_stage0 + sx * G::kStageBytes;
-                    if (issues && i >= kStages && !dead && !mbar_wait_bounded(ebars + sx * 8, ((cur / kStages) - 1u) & 1u, err)) { dead = true; atomicExch(err, 3); }
+                    if (has && !dead && !mbar_wait_bounded(ebars + sx * 8, ((cur / kStages) + 1u) & 1u, err)) { dead = true; atomicExch(err, 3); }   // the first time round the wait is for the phase before the first: over at once
+                    __syncwarp();
                     if (K8) {
-                        __syncwarp();
                         reinterpret_cast<uint32_t*>(smem + G::kOffScale)[(ring * kStages + sx) * 32 + lane] = (uint32_t)sc8[j][0] | (uint32_t)sc8[j][1] << 16;
                         __syncwarp();   // the arrival below publishes them
                     }
-                    if (issues) {
+                    if (has) {
                         mbar_arrive_expect_tx(bar, (uint32_t)G::kStageBytes);
 #pragma unroll
                         for (int x = 0; x < NK; x++) {
                             if (x && p.groups_per_box == NK) break;
-                            const int grp = (int)((p.layer_row0 + ((int64_t)pg[j][x] << p.page_shift) + ((first_slot(i) + 16 * x) & mask)) >> 4);
-                            tma_load_5d(dst + x * G::kGroupBytes, &tm_k, 0, 0, 0, grp, kvh, bar); tma_load_5d(dst + G::kHalfBytes + x * G::kGroupBytes, &tm_v, 0, 0, 0, grp, kvh, bar);
+                            const int grp = (int)((p.layer_row0 + ((int64_t)pg[j][x] << p.page_shift) + ((first_slot(sg, i) + 16 * x) & mask)) >> 4);
+                            tma_load_5d(dst + x * G::kGroupBytes, &tm_k, 0, 0, 0, grp, sg.kvh, bar); tma_load_5d(dst + G::kHalfBytes + x * G::kGroupBytes, &tm_v, 0, 0, 0, grp, sg.kvh, bar);
                         }
-                        load_pages(i + 3, pg[j]);   // behind the ring's last tile: the last page again
+                        load_pages(sg, i + 3, pg[j]);   // behind the ring's last tile: the last page again
                     }
-                    if (K8) { load_scales(i + 3, spg[j], sc8[j]); spg[j] = scale_page(i + 6); }
+                    if (K8) { load_scales(sg, i + 3, spg[j], sc8[j]); spg[j] = scale_page(sg, i + 6); }
                 }
-        } else {
-            // ---- the query block (rows t * group + j, zero behind the last; int8: columns permuted inside each 16-dim block)
-            for (int ch = tid; ch < NR * 8 * (HD / 8); ch += 384) {
-                const int r = ch / (HD / 8), c16 = ch % (HD / 8); uint4 v = make_uint4(0, 0, 0, 0);
-                if (r < rows) { const int t = r / p.group, j = r - t * p.group; v = *reinterpret_cast<const uint4*>(q16 + (((int64_t)b * p.tok_stride + p.tok0 + t) * (kvh_n * p.group) + kvh * p.group + j) * HD + c16 * 8); }
-                stage_q_chunk<K8>(smem + r * G::kQStride, c16, v);
             }
-            asm volatile("bar.sync 1, 384;" ::: "memory");   // the twelve score and value warps: the producers are under way already
+            __syncwarp();
+            if (!more) break;
+            it += (uint32_t)sg.n_mine; sg = next;
+#pragma unroll
+            for (int j = 0; j < 3; j++) {
+                pg[j][0] = npg[j][0]; pg[j][1] = npg[j][1];
+                if (K8) { spg[j] = nspg[j]; sc8[j][0] = nsc8[j][0]; sc8[j][1] = nsc8[j][1]; }
+            }
+        }
+        return;
+    }
 
-            if (h == 0) {
-                RowsState<NR> ss; int lim[NR][2]; uint32_t qf[HD / 16][2];
+    while (tile < tile_end) {
+        while (p.tile_start[b + 1] <= tile) b++;
+        const int nt = plan_ntiles(p, b), kvh = (tile - p.tile_start[b]) / nt, lt0 = (tile - p.tile_start[b]) - kvh * nt;
+        const int seg_first = tile - lt0, seg_end = seg_first + nt, my_end = min(tile_end, seg_end), n_here = my_end - tile;
+        const int kend = p.kend[b];
+        const int n_mine = n_here > ring ? (n_here - ring + kRings - 1) / kRings : 0;   // this ring's tiles: lt0 + ring, lt0 + ring + 4, ...
+        const uint32_t it_seg = it, sums = n_segs % G::kSums, sums_par = (n_segs / G::kSums) & 1u;
+        float* ml_seg = sm_ml + sums * kRings * 32;
+        const int all_see = kend - p.T + 1;   // slots below this are seen by every row (columns that hold no query too: nobody reads what they get)
+
+        if (h == 0) {
+            // ---- score warps. The query block first: rows t * group + j, zero behind the last; int8: columns permuted inside each 16-dim block
+            constexpr int kQLoads = NR * 8 * (HD / 8) / 128; uint4 qv[kQLoads];
 #pragma unroll
-                for (int nr = 0; nr < NR; nr++)
+            for (int x = 0; x < kQLoads; x++) {
+                const int ch = tid + x * 128, r = ch / (HD / 8), c16 = ch % (HD / 8), t = r / p.group, j = r - t * p.group;
+                qv[x] = r < rows ? *reinterpret_cast<const uint4*>(q16 + (((int64_t)b * p.tok_stride + p.tok0 + t) * (kvh_n * p.group) + kvh * p.group + j) * HD + c16 * 8) : make_uint4(0, 0, 0, 0);
+            }
+            score_sync();   // the block before has been read
 #pragma unroll
-                    for (int e = 0; e < 2; e++) { const int r = nr * 8 + 2 * t4 + e; ss.m[nr][e] = -INFINITY; ss.l[nr][e] = 0.0f; lim[nr][e] = r < rows ? kend - p.T + 1 + r / p.group : 0; }   // the row sees slots below this (none, when 0 or less)
-                if (NR == 1) {
+            for (int x = 0; x < kQLoads; x++) { const int ch = tid + x * 128; stage_q_chunk<K8>(smem + ch / (HD / 8) * G::kQStride, ch % (HD / 8), qv[x]); }
+            score_sync();
+            if (!dead && !mbar_wait_bounded(sempty + sums * 8, sums_par ^ 1u, err)) { dead = true; atomicExch(err, 6); }   // the sums of kSums segments ago have been read
+            RowsState<NR> ss; int lim[NR][2]; uint32_t qf[HD / 16][2];
 #pragma unroll
-                    for (int kk = 0; kk < HD / 16; kk += 2) q_frags(sm_base, G::kQStride, 0, kk, lane, qf[kk], qf[kk + 1]);
-                }
-                for (int i = 0; i < n_mine; i++) {
-                    const uint32_t cur = it_seg + (uint32_t)i, stg = cur % kStages, par = (cur / kStages) & 1u, slot = cur & 1u;
-                    const int key0 = (lt0 + ring + i * kRings) * kTile;
-                    // a wait that runs out is recorded once; afterwards waits are skipped, the control flow and every arrival stay as they are
-                    if (!dead && !mbar_wait_bounded(bars + stg * 8, par, err)) { dead = true; atomicExch(err, 1); }
-                    uint32_t sc[NK][2]; float ks[NK][2];   // K scale in the low half, V scale in the high half, of slots 16 * sb + g and 8 further
+            for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) { const int r = nr * 8 + 2 * t4 + e; ss.m[nr][e] = -INFINITY; ss.l[nr][e] = 0.0f; lim[nr][e] = r < rows ? kend - p.T + 1 + r / p.group : 0; }   // the row sees slots below this (none, when 0 or less)
+            if (NR == 1) {
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; kk += 2) q_frags(sm_base, G::kQStride, 0, kk, lane, qf[kk], qf[kk + 1]);
+            }
+            for (int i = 0; i < n_mine; i++) {
+                const uint32_t cur = it_seg + (uint32_t)i, stg = cur % kStages, par = (cur / kStages) & 1u, slot = cur & 1u;
+                const int key0 = (lt0 + ring + i * kRings) * kTile;
+                // a wait that runs out is recorded once; afterwards waits are skipped, the control flow and every arrival stay as they are
+                if (!dead && !mbar_wait_bounded(bars + stg * 8, par, err)) { dead = true; atomicExch(err, 1); }
+                uint32_t sc[NK][2]; float ks[NK][2];   // K scale in the low half, V scale in the high half, of slots 16 * sb + g and 8 further
+#pragma unroll
+                for (int sb = 0; sb < NK; sb++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        if (K8) sc[sb][e] = *reinterpret_cast<const uint32_t*>(smem + G::kOffScale + (ring * kStages + stg) * 128 + (16 * sb + 8 * e + g) * 4);
+                        ks[sb][e] = K8 ? __half2float(__ushort_as_half((unsigned short)sc[sb][e])) : 1.0f;
+                    }
+                float s[NK][NR][4], al[NR][2];
+                paged_scores<HD, K8, NR>(sm_base, ring_stage0 + stg * G::kStageBytes, qf, ks, lane, s);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(ebars + stg * 8);   // K and the scales (in registers by now) of this stage are no longer needed
+                if (key0 + kTile > all_see) {   // masked by select: what lies behind the last slot may be anything
 #pragma unroll
                     for (int sb = 0; sb < NK; sb++)
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            if (K8) sc[sb][e] = *reinterpret_cast<const uint32_t*>(smem + G::kOffScale + (ring * kStages + stg) * 128 + (16 * sb + 8 * e + g) * 4);
-                            ks[sb][e] = K8 ? __half2float(__ushort_as_half((unsigned short)sc[sb][e])) : 1.0f;
+                        for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) if (key0 + 16 * sb + 8 * (e >> 1) + g >= lim[nr][e & 1]) s[sb][nr][e] = -INFINITY;
+                }
+                if (scores) {   // [tile of the list][slot][8 or 16 rows]: full 32-byte sectors
+                    float* st = scores + ((int64_t)(tile + ring + i * kRings) * kTile + g) * srow + 2 * t4;
+#pragma unroll
+                    for (int sb = 0; sb < NK; sb++)
+#pragma unroll
+                        for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) *reinterpret_cast<float2*>(st + (16 * sb + 8 * e) * srow + nr * 8) = make_float2(s[sb][nr][2 * e], s[sb][nr][2 * e + 1]);
+                }
+                paged_softmax<NK, NR, G::kPShift>(s, ss, al);
+                if (K8) {
+#pragma unroll
+                    for (int sb = 0; sb < NK; sb++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float v = __half2float(__ushort_as_half((unsigned short)(sc[sb][e >> 1] >> 16)));
+#pragma unroll
+                            for (int nr = 0; nr < NR; nr++) s[sb][nr][e] *= v;
                         }
-                    float s[NK][NR][4], al[NR][2];
-                    paged_scores<HD, K8, NR>(sm_base, ring_stage0 + stg * G::kStageBytes, qf, ks, lane, s);
+                }
+                if (cur >= 2 && !dead && !mbar_wait_bounded(pempty + slot * 8, ((cur >> 1) - 1u) & 1u, err)) { dead = true; atomicExch(err, 4); }
+                paged_publish<HD, K8, NR>(sm_base + p_off + slot * G::kPBytes, reinterpret_cast<float*>(smem + p_off + (slot + 1) * G::kPBytes - 64), s, al, p.two_terms, lane);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(pfull + slot * 8);
+            }
+#pragma unroll
+            for (int nr = 0; nr < NR; nr++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    float l = ss.l[nr][e];
+                    l += __shfl_xor_sync(0xffffffffu, l, 4); l += __shfl_xor_sync(0xffffffffu, l, 8); l += __shfl_xor_sync(0xffffffffu, l, 16);
+                    if (g == 0) *reinterpret_cast<float2*>(ml_seg + (ring * 16 + nr * 8 + 2 * t4 + e) * 2) = make_float2(ss.m[nr][e], l);
+                }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sfull + sums * 8);
+        } else {
+            const int vh = h - 1; ValueAcc<HD, NR> vst; vst.clear();
+            for (int i = 0; i < n_mine; i++) {
+                const uint32_t cur = it_seg + (uint32_t)i, stg = cur % kStages, par = (cur / kStages) & 1u, slot = cur & 1u;
+                const uint32_t vt = ring_stage0 + stg * G::kStageBytes + G::kHalfBytes;
+                const int key0 = (lt0 + ring + i * kRings) * kTile;
+                if (!dead && !mbar_wait_bounded(bars + stg * 8, par, err)) { dead = true; atomicExch(err, 1); }
+                if (!K8 && key0 + kTile > kend) {   // the V rows behind the last slot become zeros (0 x NaN is not 0; int8 codes are finite whatever they are)
+                    const int nk = max(0, kend - key0);
+                    constexpr int kHC = G::kRowBytes / 32;   // 16-byte chunks of half a head row
+                    for (int idx = lane; idx < (kTile - nk) * kHC; idx += 32) {
+                        const int r = nk + idx / kHC, c = vh * kHC + idx % kHC;
+                        *reinterpret_cast<uint4*>(smem + (vt - sm_base) + (r >> 4) * G::kGroupBytes + (c >> 3) * 2048 + (r & 15) * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async();   // generic writes to a stage that TMA fills again
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(ebars + stg * 8);   // K and the scales (in registers by now) of this stage are no longer needed
-                    if (key0 + kTile > all_see) {   // masked by select: what lies behind the last slot may be anything
+                }
+                if (!dead && !mbar_wait_bounded(pfull + slot * 8, (cur >> 1) & 1u, err)) { dead = true; atomicExch(err, 5); }
+                const float* alpha = reinterpret_cast<const float*>(smem + p_off + (slot + 1) * G::kPBytes - 64);
+                if (!K8 || p.two_terms) paged_values<HD, K8, NR, true>(vt, sm_base + p_off + slot * G::kPBytes, alpha, vst, lane, vh); else paged_values<HD, K8, NR, false>(vt, sm_base + p_off + slot * G::kPBytes, alpha, vst, lane, vh);
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(pempty + slot * 8); mbar_arrive(ebars + stg * 8); }
+            }
+            // ---- join the four rings: ring 3 leaves its rows of O^T, scaled to the joint maximum, where the P slots were, ring 2 adds its own, ring 1, ring 0. The same lane holds the same
+            // dims and rows in every ring, and the order is fixed. The producers are in the next segment meanwhile.
+            if (!dead && !mbar_wait_bounded(sfull + sums * 8, sums_par, err)) { dead = true; atomicExch(err, 7); }   // the rings' (m, l) are there
+            value_sync();   // the segment before has left the block (NR = 2: and P is read)
 #pragma unroll
-                        for (int sb = 0; sb < NK; sb++)
+            for (int nr = 0; nr < NR; nr++)
 #pragma unroll
-                            for (int nr = 0; nr < NR; nr++)
+                for (int e = 0; e < 2; e++) {
+                    const int r = nr * 8 + 2 * t4 + e; float mx = -INFINITY, l = 0.0f, mine = 0.0f;
 #pragma unroll
-                                for (int e = 0; e < 4; e++) if (key0 + 16 * sb + 8 * (e >> 1) + g >= lim[nr][e & 1]) s[sb][nr][e] = -INFINITY;
+                    for (int ww = 0; ww < kRings; ww++) mx = fmaxf(mx, ml_seg[(ww * 16 + r) * 2]);
+#pragma unroll
+                    for (int ww = 0; ww < kRings; ww++) {
+                        const float mm = ml_seg[(ww * 16 + r) * 2], wt = mm == -INFINITY ? 0.0f : ex2(mm - mx);
+                        l += ml_seg[(ww * 16 + r) * 2 + 1] * wt;
+                        if (ww == ring) mine = wt;
                     }
-                    if (scores) {   // [tile of the list][slot][8 or 16 rows]: full 32-byte sectors
-                        float* st = scores + ((int64_t)(tile + ring + i * kRings) * kTile + g) * srow + 2 * t4;
+                    if (ring == 0 && vh == 0 && g == 0) *reinterpret_cast<float2*>(joined_ml + r * 2) = make_float2(mx, l);
 #pragma unroll
-                        for (int sb = 0; sb < NK; sb++)
+                    for (int j = 0; j < HD / 32; j++) { vst.o[j][nr][e] = mine == 0.0f ? 0.0f : vst.o[j][nr][e] * mine; vst.o[j][nr][2 + e] = mine == 0.0f ? 0.0f : vst.o[j][nr][2 + e] * mine; }
+                }
+            float* mine = red + vh * G::kAcc * 32 + lane;   // [half][accumulator][lane]
+#pragma unroll 1
+            for (int from = kRings - 1; from >= 0; from--) {
+                if (ring == from) {
 #pragma unroll
-                            for (int nr = 0; nr < NR; nr++)
+                    for (int j = 0; j < HD / 32; j++)
 #pragma unroll
-                                for (int e = 0; e < 2; e++) *reinterpret_cast<float2*>(st + (16 * sb + 8 * e) * srow + nr * 8) = make_float2(s[sb][nr][2 * e], s[sb][nr][2 * e + 1]);
-                    }
-                    paged_softmax<NK, NR, G::kPShift>(s, ss, al);
-                    if (K8) {
-#pragma unroll
-                        for (int sb = 0; sb < NK; sb++)
+                        for (int nr = 0; nr < NR; nr++)
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                const float v = __half2float(__ushort_as_half((unsigned short)(sc[sb][e >> 1] >> 16)));
-#pragma unroll
-                                for (int nr = 0; nr < NR; nr++) s[sb][nr][e] *= v;
+                                float* at = mine + ((j * NR + nr) * 4 + e) * 32;
+                                *at = (from == kRings - 1 ? 0.0f : *at) + vst.o[j][nr][e];
                             }
-                    }
-                    if (cur >= 2 && !dead && !mbar_wait_bounded(pempty + slot * 8, ((cur >> 1) - 1u) & 1u, err)) { dead = true; atomicExch(err, 4); }
-                    paged_publish<HD, K8, NR>(sm_base + p_off + slot * G::kPBytes, reinterpret_cast<float*>(smem + p_off + (slot + 1) * G::kPBytes - 64), s, al, p.two_terms, lane);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(pfull + slot * 8);
                 }
+                if (from) asm volatile("bar.sync %0, 128;" ::"r"(3 + vh) : "memory");   // the four value warps of this half
+            }
+            value_sync();   // the CTA's rows are there
+            // ---- final rows, or a partial
+            const int seg = b * kvh_n + kvh;
+            const bool whole = n_here == nt;
+            constexpr int kTpr = HD / 2, kRowPar = 256 / kTpr;   // threads per row (two dims each), rows at a time
+            const int vtid = tid - 128, d0 = 2 * (vtid % kTpr), dx = d0 & 15;
+            const float* from = red + ((d0 / (HD / 2)) * G::kAcc + (d0 % (HD / 2)) / 16 * NR * 4 + (K8 ? 0 : dx >> 3) * 2) * 32 + (K8 ? dx >> 1 : dx & 7) * 4;   // of d0; d0 + 1 lies two accumulators (int8) or four lanes further
+            constexpr int kIters = NR * 8 / kRowPar; const int r0 = vtid / kTpr;
+            if (whole) {
+                float2 gate[kIters];   // requested together
 #pragma unroll
-                for (int nr = 0; nr < NR; nr++)
+                for (int x = 0; x < kIters; x++) if (r0 + x * kRowPar < rows) gate[x] = paged_gate(o, paged_out_at<HD>(p, b, kvh, r0 + x * kRowPar, d0));
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float l = ss.l[nr][e];
-                        l += __shfl_xor_sync(0xffffffffu, l, 4); l += __shfl_xor_sync(0xffffffffu, l, 8); l += __shfl_xor_sync(0xffffffffu, l, 16);
-                        if (g == 0) *reinterpret_cast<float2*>(sm_ml + (ring * 16 + nr * 8 + 2 * t4 + e) * 2) = make_float2(ss.m[nr][e], l);
-                    }
-            } else {
-                const int vh = h - 1; ValueAcc<HD, NR> vst; vst.clear();
-                for (int i = 0; i < n_mine; i++) {
-                    const uint32_t cur = it_seg + (uint32_t)i, stg = cur % kStages, par = (cur / kStages) & 1u, slot = cur & 1u;
-                    const uint32_t vt = ring_stage0 + stg * G::kStageBytes + G::kHalfBytes;
-                    const int key0 = (lt0 + ring + i * kRings) * kTile;
-                    if (!dead && !mbar_wait_bounded(bars + stg * 8, par, err)) { dead = true; atomicExch(err, 1); }
-                    if (!K8 && key0 + kTile > kend) {   // the V rows behind the last slot become zeros (0 x NaN is not 0; int8 codes are finite whatever they are)
-                        const int nk = max(0, kend - key0);
-                        constexpr int kHC = G::kRowBytes / 32;   // 16-byte chunks of half a head row
-                        for (int idx = lane; idx < (kTile - nk) * kHC; idx += 32) {
-                            const int r = nk + idx / kHC, c = vh * kHC + idx % kHC;
-                            *reinterpret_cast<uint4*>(smem + (vt - sm_base) + (r >> 4) * G::kGroupBytes + (c >> 3) * 2048 + (r & 15) * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_proxy_async();   // generic writes to a stage that TMA fills again
-                        __syncwarp();
-                    }
-                    if (!dead && !mbar_wait_bounded(pfull + slot * 8, (cur >> 1) & 1u, err)) { dead = true; atomicExch(err, 5); }
-                    const float* alpha = reinterpret_cast<const float*>(smem + p_off + (slot + 1) * G::kPBytes - 64);
-                    if (!K8 || p.two_terms) paged_values<HD, K8, NR, true>(vt, sm_base + p_off + slot * G::kPBytes, alpha, vst, lane, vh); else paged_values<HD, K8, NR, false>(vt, sm_base + p_off + slot * G::kPBytes, alpha, vst, lane, vh);
-                    __syncwarp();
-                    if (lane == 0) { mbar_arrive(pempty + slot * 8); mbar_arrive(ebars + stg * 8); }
+                for (int x = 0; x < kIters; x++) {
+                    const int r = r0 + x * kRowPar; const float* at = from + ((r >> 3) * 4 + (r & 1)) * 32 + ((r & 7) >> 1);
+                    if (r < rows) paged_emit(p, o, b, kvh, r, d0, paged_out_at<HD>(p, b, kvh, r, d0), gate[x], joined_ml[r * 2], joined_ml[r * 2 + 1], at[0], at[K8 ? 64 : 4]);
                 }
-                asm volatile("bar.sync %0, 64;" ::"r"(2 + ring) : "memory");   // both value warps are done with the ring's stages (and so is the score warp, whose last P they have used): the rows of O go there
-                float* mo = reinterpret_cast<float*>(smem + stage_off + ring * G::kRingBytes);
-#pragma unroll
-                for (int j = 0; j < HD / 32; j++)
-#pragma unroll
-                    for (int nr = 0; nr < NR; nr++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) mo[(nr * 8 + 2 * t4 + (e & 1)) * G::kMergeStride + vh * (HD / 2) + 16 * j + (K8 ? 2 * g + (e >> 1) : g + 8 * (e >> 1))] = vst.o[j][nr][e];
+            } else {   // (CTA, segment) pairs have CTA + segment of their own
+                const int64_t sl = blockIdx.x + seg;
+                for (int r = r0; r < rows; r += kRowPar) {
+                    const float* at = from + ((r >> 3) * 4 + (r & 1)) * 32 + ((r & 7) >> 1);
+                    *reinterpret_cast<float2*>(scratch_o + sl * (16 * HD) + r * HD + d0) = make_float2(at[0], at[K8 ? 64 : 4]);
+                    if (d0 == 0) *reinterpret_cast<float2*>(scratch_ml + sl * 32 + r * 2) = make_float2(joined_ml[r * 2], joined_ml[r * 2 + 1]);
+                }
             }
-        }
-        it = it_seg + (uint32_t)n_mine;
-
-        // ---- join the four rings (every tile issued has been waited for: no copy is in flight)
-        __syncthreads();
-        constexpr int kTpr = HD / 2, kRowPar = 384 / kTpr;   // threads per row (two dims each), rows at a time over the twelve ring warps
-        const int seg = b * kvh_n + kvh, c_first = plan_cta_of_tile(p, seg_first), n_contrib = plan_cta_of_tile(p, seg_end - 1) - c_first + 1;
-        const int d0 = 2 * (tid % kTpr), rsel = h < 3 ? tid / kTpr : rows; const bool whole = n_contrib == 1;
-        float* slot_o = scratch_o + (int64_t)(blockIdx.x + seg) * (16 * HD); float* slot_ml = scratch_ml + (int64_t)(blockIdx.x + seg) * 32;   // (CTA, segment) pairs have CTA + segment of their own
-        for (int r = rsel; r < rows; r += kRowPar) {
-            float M = -INFINITY, L = 0.0f, A0 = 0.0f, A1 = 0.0f;
-#pragma unroll
-            for (int ww = 0; ww < kRings; ww++) M = fmaxf(M, sm_ml[(ww * 16 + r) * 2]);
-#pragma unroll
-            for (int ww = 0; ww < kRings; ww++) {
-                const float mm = sm_ml[(ww * 16 + r) * 2], wt = (mm == -INFINITY) ? 0.0f : ex2(mm - M);
-                const float* src = reinterpret_cast<const float*>(smem + stage_off + ww * G::kRingBytes) + r * G::kMergeStride + d0;
-                L += sm_ml[(ww * 16 + r) * 2 + 1] * wt;
-                if (wt != 0.0f) { A0 += src[0] * wt; A1 += src[1] * wt; }
-            }
-            if (whole) paged_emit<HD>(p, o, b, kvh, r, d0, M, L, A0, A1);
-            else { *reinterpret_cast<float2*>(slot_o + r * HD + d0) = make_float2(A0, A1); if (d0 == 0) { slot_ml[r * 2] = M; slot_ml[r * 2 + 1] = L; } }
-        }
-        if (!whole && p.merge_in_kernel) {   // the last of (at most 8) contributors joins everybody's partial rows
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) { const int old = atomicAdd(&counters[seg], 1); s_flag = (old == n_contrib - 1); }
-            __syncthreads();
-            if (s_flag) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sempty + sums * 8);
+            if (p.merge_in_kernel && !whole) {   // the last of (at most 8) contributors joins everybody's partial rows
+                const int c_first = plan_first_cta(p, blockIdx.x, seg_first), n_contrib = plan_last_cta(p, blockIdx.x, seg_end) - c_first + 1;
                 __threadfence();
-                for (int r = rsel; r < rows; r += kRowPar) {
-                    float M = -INFINITY, L = 0.0f, A0 = 0.0f, A1 = 0.0f;
-                    for (int c = 0; c < n_contrib; c++) M = fmaxf(M, __ldcg(scratch_ml + (int64_t)(c_first + c + seg) * 32 + r * 2));
-#pragma unroll 4
-                    for (int c = 0; c < n_contrib; c++) {
-                        const int64_t sl = c_first + c + seg; const float mm = __ldcg(scratch_ml + sl * 32 + r * 2), wt = (mm == -INFINITY) ? 0.0f : ex2(mm - M);
-                        const float2 oo = __ldcg(reinterpret_cast<const float2*>(scratch_o + sl * (16 * HD) + r * HD + d0));
-                        L += __ldcg(scratch_ml + sl * 32 + r * 2 + 1) * wt; A0 += oo.x * wt; A1 += oo.y * wt;
+                value_sync();
+                if (vtid == 0) { const int old = atomicAdd(&counters[seg], 1); s_flag = (old == n_contrib - 1); if (s_flag) counters[seg] = 0; }   // zero again for the next call
+                value_sync();
+                if (s_flag) {
+                    __threadfence();
+                    for (int r = r0; r < rows; r += kRowPar) {
+                        const int64_t sl = c_first + seg, at = paged_out_at<HD>(p, b, kvh, r, d0); const float2 gate = paged_gate(o, at);
+                        float2 ml[8], oo[8]; float M = -INFINITY, L = 0.0f, A0 = 0.0f, A1 = 0.0f;
+#pragma unroll
+                        for (int c = 0; c < 8; c++) {
+                            ml[c] = c < n_contrib ? __ldcg(reinterpret_cast<const float2*>(scratch_ml + (sl + c) * 32 + r * 2)) : make_float2(-INFINITY, 0.0f);
+                            oo[c] = c < n_contrib ? __ldcg(reinterpret_cast<const float2*>(scratch_o + (sl + c) * (16 * HD) + r * HD + d0)) : make_float2(0.0f, 0.0f);
+                        }
+#pragma unroll
+                        for (int c = 0; c < 8; c++) M = fmaxf(M, ml[c].x);
+#pragma unroll
+                        for (int c = 0; c < 8; c++) { const float wt = ml[c].x == -INFINITY ? 0.0f : ex2(ml[c].x - M); L += ml[c].y * wt; A0 += oo[c].x * wt; A1 += oo[c].y * wt; }
+                        paged_emit(p, o, b, kvh, r, d0, at, gate, M, L, A0, A1);
                     }
-                    paged_emit<HD>(p, o, b, kvh, r, d0, M, L, A0, A1);
                 }
-                if (tid == 0) counters[seg] = 0;   // ready for the next call
             }
         }
-        fence_proxy_async();   // the merge buffers lie in the stages that the next segment's TMA writes
-        __syncthreads();
+        it += (uint32_t)n_mine; n_segs++;
         tile = my_end;
     }
 }
@@ -522,7 +611,7 @@ __global__ void __launch_bounds__(1024) paged_combine_kernel(const __grid_consta
     constexpr int kQ = 1024 / HD, kU = 48 / kQ;
     __shared__ float s_acc[kQ][HD], s_M[kQ], s_L[kQ];
     const int r = blockIdx.x, seg = blockIdx.y, b = seg / p.kv_heads, kvh = seg - b * p.kv_heads, d = threadIdx.x % HD, q = threadIdx.x / HD;
-    const int nt = plan_ntiles(p, b), first = p.tile_start[b] + kvh * nt, c_first = plan_cta_of_tile(p, first), n_c = plan_cta_of_tile(p, first + nt - 1) - c_first + 1;
+    const int nt = plan_ntiles(p, b), seg_first = p.tile_start[b] + kvh * nt, c_first = plan_cta_of(p, seg_first), n_c = plan_cta_of(p, seg_first + nt - 1) - c_first + 1;
     pdl_wait(); pdl_launch_dependents();
     if (n_c == 1) return;   // written by its only contributor
     const float* ml = scratch_ml + (int64_t)(c_first + seg) * 32 + r * 2; const float* po = scratch_o + (int64_t)(c_first + seg) * (16 * HD) + r * HD + d;
@@ -550,7 +639,8 @@ __global__ void __launch_bounds__(1024) paged_combine_kernel(const __grid_consta
     for (int u = 0; u < kQ; u++) M = fmaxf(M, s_M[u]);
 #pragma unroll
     for (int u = 0; u < kQ; u++) { const float wt = (s_M[u] == -INFINITY) ? 0.0f : ex2(s_M[u] - M); A0 = fmaf(s_acc[u][d], wt, A0); A1 = fmaf(s_acc[u][d + 1], wt, A1); L = fmaf(s_L[u], wt, L); }
-    paged_emit<HD>(p, o, b, kvh, r, d, M, L, A0, A1);
+    const int64_t at = paged_out_at<HD>(p, b, kvh, r, d);
+    paged_emit(p, o, b, kvh, r, d, at, paged_gate(o, at), M, L, A0, A1);
 }
 
 // weight[kv head][slot] += sum over the rows of 2^(s * log2 e - m + shift) / l: the slot's final probabilities, from the scores the decode kernel
@@ -582,18 +672,43 @@ __global__ void __launch_bounds__(256) paged_weight_kernel(const __grid_constant
 
 // The work split (host only): tiles, ranges and where the partial rows are joined. p.n, p.kv_heads and p.kend are set.
 int split_paged_tiles(PagedPlan& p, int tile_keys, int sm_count) {
+    sm_count = std::min(sm_count, kMaxCtas);
     int total = 0; bool same = true;
     for (int i = 0; i < p.n; i++) {
         p.tile_start[i] = total; total += p.kv_heads * std::max(1, (p.kend[i] + tile_keys - 1) / tile_keys);   // a sequence without keys has one (masked) tile: its rows are written
         same = same && (i == 0 || total - p.tile_start[i] == p.tile_start[1]);
     }
     for (int i = p.n; i <= KATA_PAGED_MAX_BATCH; i++) p.tile_start[i] = total;
-    p.cps = 0; p.n_ctas = std::max(1, std::min(sm_count, total)); p.q_tiles = total / p.n_ctas; p.r_tiles = total % p.n_ctas;
-    // equal segments that divide nearly all SMs get CTAs of their own: none then pays for crossing into a second segment (4 to 5 us in the contiguous kernel)
-    const int n_seg = p.n * p.kv_heads, nt = plan_ntiles(p, 0), cps = n_seg <= sm_count ? std::min(sm_count / n_seg, nt) : 0;
-    if (same && cps >= 1 && (cps == nt || cps * n_seg * 100 >= sm_count * 97)) { p.cps = cps; p.n_ctas = cps * n_seg; }
+    // Equal segments that divide nearly all SMs, or whose shares are hardly longer than an even split's, get CTAs of their own: none then pays for a second segment (eight sequences of 300 slots:
+    // 128 CTAs of 5 tiles 12.7 us, 148 of 4.1 tiles 16.3 us).
+    const int n_seg = p.n * p.kv_heads, nt0 = plan_ntiles(p, 0), cps = n_seg <= sm_count ? std::min(sm_count / n_seg, nt0) : 0;
+    constexpr int kPad = 8, kSnap = 4;
     int most = 1;
-    for (int i = 0; i < p.n; i++) for (int kv = 0; kv < p.kv_heads; kv++) { const int n = plan_ntiles(p, i), f = p.tile_start[i] + kv * n; most = std::max(most, plan_cta_of_tile(p, f + n - 1) - plan_cta_of_tile(p, f) + 1); }
+    if (same && cps >= 1 && (cps * n_seg * 100 >= sm_count * 97 || (nt0 + cps - 1) / cps <= total / sm_count + kPad)) {
+        p.n_ctas = cps * n_seg; most = cps;
+        for (int c = 0; c < p.n_ctas; c++) p.cut[c] = c / cps * nt0 + (int)((int64_t)nt0 * (c % cps) / cps);
+        p.cut[p.n_ctas] = total;
+    } else {
+        // A segment costs a CTA more than its tiles: its rows are joined and written, the next one's query staged, some 3 us beside 0.37 us a tile. Many short segments would pile up in a few CTAs
+        // (32 int8 sequences of 300 to 32K slots, sorted by length: 218 us, 182 like this): each counts as kPad tiles more, where the ranges are long enough for that. A cut that falls within kSnap tiles of an
+        // end of a segment moves there: less than what the second piece would cost.
+        p.n_ctas = std::max(1, std::min(sm_count, total));
+        const int pad = total >= (int64_t)sm_count * 4 * kPad ? kPad : 0, snap = pad ? kSnap : 0; const int64_t places = total + (int64_t)n_seg * pad;
+        int c = 0; int64_t place = 0;   // of the segment: its pad, then its tiles
+        for (int i = 0; i < p.n; i++) {
+            const int nt = plan_ntiles(p, i);
+            for (int kv = 0; kv < p.kv_heads; kv++, place += nt + pad) {
+                int cuts_inside = 0;
+                for (; c < p.n_ctas && places * c / p.n_ctas < place + nt + pad; c++) {
+                    int in = (int)(places * c / p.n_ctas - place) - pad;
+                    in = in <= snap ? 0 : in >= nt - snap ? nt : in;
+                    p.cut[c] = p.tile_start[i] + kv * nt + in; cuts_inside += in > 0 && in < nt;
+                }
+                most = std::max(most, cuts_inside + 1);
+            }
+        }
+        p.cut[p.n_ctas] = total;
+    }
     p.merge_in_kernel = most <= 8;   // few contributors: the last one joins them (no second kernel); many: one SM would pull them all, a grid does it in one round trip
     return most;
 }
@@ -609,7 +724,7 @@ size_t paged_part_ml_floats(const PagedCtx& c) { return (size_t)(c.sm_count + KA
 
 cudaError_t configure_paged_decode(const PagedCtx& c) {   // shared-memory opt-in, per device
     cudaError_t e = cudaSuccess;
-#define X(HD, K8, NR) if (e == cudaSuccess && c.cfg.head_dim == HD && c.int8() == K8) e = cudaFuncSetAttribute(paged_decode_kernel<HD, K8, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, PGeo<HD, K8>::kSmem);
+#define X(HD, K8, NR) if (e == cudaSuccess && c.cfg.head_dim == HD && c.int8() == K8) e = cudaFuncSetAttribute(paged_decode_kernel<HD, K8, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, PGeo<HD, K8, NR>::kSmem);
     KATA_PAGED_KERNELS(X)
 #undef X
     return e;
@@ -626,7 +741,7 @@ cudaError_t launch_paged_decode(PagedCtx& c, int layer, int n, const int32_t* se
         const PagedOut o{gate, out, out_dtype, accumulate ? c.fin_ml : nullptr}; float* scores = accumulate ? c.scores : nullptr;
         if (accumulate && p.tile_start[n] > c.score_tiles) return cudaErrorInvalidValue;   // cannot be: the pool bounds the tiles
         cudaError_t e = cudaErrorInvalidValue;
-#define X(HD, K8, NR) if (hd == HD && c.int8() == K8 && (c.group * p.T > 8) == (NR == 2)) e = launch_pdl(paged_decode_kernel<HD, K8, NR>, dim3(p.n_ctas), dim3(PGeo<HD, K8>::kThreads), PGeo<HD, K8>::kSmem, s, c.tm_k, c.tm_v, p, (const int32_t*)c.d_table, q16, o, \
+#define X(HD, K8, NR) if (hd == HD && c.int8() == K8 && (c.group * p.T > 8) == (NR == 2)) e = launch_pdl(paged_decode_kernel<HD, K8, NR>, dim3(p.n_ctas), dim3(PGeo<HD, K8, NR>::kThreads), PGeo<HD, K8, NR>::kSmem, s, c.tm_k, c.tm_v, p, (const int32_t*)c.d_table, q16, o, \
             (const __half*)c.layer_plane(KATA_PAGED_K_SCALE, layer), (const __half*)c.layer_plane(KATA_PAGED_V_SCALE, layer), scores, c.part_o, c.part_ml, c.counters, c.d_err);
         KATA_PAGED_KERNELS(X)
 #undef X
@@ -641,7 +756,7 @@ cudaError_t launch_paged_decode(PagedCtx& c, int layer, int n, const int32_t* se
         if (accumulate) {
             const int64_t keys = (int64_t)p.tile_start[n] * tile_keys;
             e = launch_pdl(paged_weight_kernel, dim3((unsigned)((keys + 255) / 256)), dim3(256), 0, s, p, (const int32_t*)c.d_table, (const float*)c.scores, (const float*)c.fin_ml, (float*)c.layer_plane(KATA_PAGED_WEIGHT, layer),
-                           tile_keys == 16 ? 4 : 5, c.int8() ? (float)PGeo<256, true>::kPShift : (float)PGeo<256, false>::kPShift);
+                           tile_keys == 16 ? 4 : 5, c.int8() ? (float)PGeo<256, true, 1>::kPShift : (float)PGeo<256, false, 1>::kPShift);
             if (e != cudaSuccess) return e;
             c.launches++;
         }
@@ -658,7 +773,11 @@ extern "C" int kata_paged_decode_plan(int32_t n, const int32_t* n_keys, int32_t 
     for (int i = 0; i < n; i++) { if (n_keys[i] < 0 || n_keys[i] > KATA_PAGED_MAX_SLOTS) return -1; p.kend[i] = n_keys[i]; }
     *max_contrib = split_paged_tiles(p, tile_keys, sm_count);
     if (p.n_ctas + 1 > first_tile_cap) return -1;
-    for (int cta = 0; cta <= p.n_ctas; cta++) first_tile[cta] = plan_first_tile(p, cta);
-    for (int cta = 0; cta < p.n_ctas; cta++) for (int t = first_tile[cta]; t < first_tile[cta + 1]; t++) if (plan_cta_of_tile(p, t) != cta) return -2;   // the two maps disagree
+    for (int cta = 0; cta <= p.n_ctas; cta++) first_tile[cta] = p.cut[cta];
+    for (int i = 0, cta = 0; i < n; i++) for (int kv = 0; kv < kv_heads; kv++) for (int lt = 0; lt < plan_ntiles(p, i); lt++) {
+        const int nt = plan_ntiles(p, i), first = p.tile_start[i] + kv * nt, t = first + lt;
+        while (p.cut[cta + 1] <= t) cta++;
+        if (plan_cta_of(p, t) != cta || plan_first_cta(p, cta, first) != plan_cta_of(p, first) || plan_last_cta(p, cta, first + nt) != plan_cta_of(p, first + nt - 1)) return -2;   // the maps disagree
+    }
     return p.n_ctas;
 }
