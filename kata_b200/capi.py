@@ -25,7 +25,7 @@ QD, KVD, QFULL, MAX_BATCH = 6144, 1024, 12288, 64
 
 EXPORTS = [
     "kata_attn_create", "kata_attn_destroy", "kata_attn_reset", "kata_attn_numerics_tag", "kata_attn_last_error", "kata_attn_check",
-    "kata_attn_prep", "kata_attn_kv_quant", "kata_attn_decode", "kata_attn_decode_scalar", "kata_attn_prefill",
+    "kata_attn_prep", "kata_attn_prep_axes", "kata_attn_kv_quant", "kata_attn_decode", "kata_attn_decode_scalar", "kata_attn_prefill",
     "kata_attn_decode_partial", "kata_attn_merge_parts", "kata_attn_kv_planes", "kata_attn_kv_plane_row_bytes",
     "kata_attn_kv_plane_read", "kata_attn_kv_plane_write", "kata_attn_kv_plane_ptr", "kata_attn_mark_rows_written", "kata_attn_launch_count", "kata_attn_decode_static", "kata_attn_decode_static_check", "kata_attn_set_position_offset", "kata_attn_set_kv_heads", "kata_attn_out_fwht",
     "kata_attn_layers_step", "kata_attn_layers_decode", "kata_attn_prefill_plan", "kata_attn_decode_plan", "kata_attn_host_step_create", "kata_attn_host_step_destroy", "kata_attn_host_step_run",
@@ -166,6 +166,21 @@ class AttnContext:
                 q32 = torch.empty((n, T, QD), dtype=torch.float32, device=dev)
         self._ck(self.L.kata_attn_prep(self.h, layer, n, sp, pp, T, _dp(qfull), _dp(kproj), _dp(vproj), act, _dp(qnorm), _dp(knorm),
                                        _dp(q16), _dp(q32), _dp(gate), h0, nh, _stream()))
+        return q16, q32, gate
+
+    def prep_axes(self, layer, seq_ids, pos0, T, axis_pos, sections, qfull, kproj, vproj, qnorm, knorm, interleaved=False, h0=0, nh=32, q16=None, q32=None, gate=None):
+        """As prep, with rotary positions of three axes: axis_pos int32 [n][T][3] on the device, sections the frequencies per axis (sum 32) (kata_attn_prep_axes)."""
+        sa, sp = _i32(seq_ids)
+        pa, pp = _i32(pos0)
+        n, ref = len(sa), kproj if kproj is not None else qfull
+        if axis_pos.dtype != torch.int32 or axis_pos.numel() != n * T * 3 or not axis_pos.is_contiguous() or axis_pos.device != ref.device or len(sections) != 3:
+            raise ValueError(f"axis_pos: a contiguous int32 tensor [{n}][{T}][3] on {ref.device} and three sections are needed")
+        if h0 < 24:
+            q16 = torch.empty((n, T, QD), dtype=torch.float16, device=ref.device) if q16 is None else q16
+            gate = torch.empty((n, T, QD), dtype=torch.float32, device=ref.device) if gate is None else gate
+        xa, xp = _i32(sections)
+        self._ck(self.L.kata_attn_prep_axes(self.h, layer, n, sp, pp, T, _dp(axis_pos), xp, 1 if interleaved else 0, _dp(qfull), _dp(kproj), _dp(vproj), _ACT[ref.dtype],
+                                            _dp(qnorm), _dp(knorm), _dp(q16), _dp(q32), _dp(gate), h0, nh, _stream()))
         return q16, q32, gate
 
     def layers_step(self, n_layers, seq_ids, pos0, T, qfull, kproj, vproj, qnorm, knorm, q16, gate, out, first_pos=0):

@@ -169,10 +169,9 @@ int kata_attn_check(kata_attn_ctx* h, void* stream) {
     return KATA_OK;
 }
 
-int kata_attn_prep(kata_attn_ctx* h, int32_t layer, int32_t n, const int32_t* seq_ids, const int32_t* pos0, int32_t T,
-                   const void* d_qfull, const void* d_kproj, const void* d_vproj, int32_t act_dtype,
-                   const float* d_qnorm, const float* d_knorm, void* d_q16, float* d_q32, float* d_gate, int32_t h0, int32_t nh, void* stream) {
-    if (!h) return KATA_ERR_ARG;
+static int prep_call(kata_attn_ctx* h, int32_t layer, int32_t n, const int32_t* seq_ids, const int32_t* pos0, int32_t T, const int32_t* d_axis_pos, uint64_t axes,
+                     const void* d_qfull, const void* d_kproj, const void* d_vproj, int32_t act_dtype,
+                     const float* d_qnorm, const float* d_knorm, void* d_q16, float* d_q32, float* d_gate, int32_t h0, int32_t nh, void* stream) {
     Ctx& c = h->c;
     if (T < 1 || T > KATA_MAX_CHUNK) return fail(c, KATA_ERR_RANGE, "prep of %d tokens (1..%d)", T, KATA_MAX_CHUNK);
     if (h0 < 0 || nh < 1 || h0 + nh > 32) return fail(c, KATA_ERR_ARG, "head slots [%d,%d) outside [0,32)", h0, h0 + nh);
@@ -181,10 +180,28 @@ int kata_attn_prep(kata_attn_ctx* h, int32_t layer, int32_t n, const int32_t* se
     if ((hasQ && (!d_qfull || !d_qnorm)) || (hasK && (!d_kproj || !d_knorm)) || (hasV && !d_vproj)) return fail(c, KATA_ERR_ARG, "a projection or norm weight needed by head slots [%d,%d) is null", h0, h0 + nh);
     kata::Batch b{}; if (int rc = make_batch(c, layer, n, seq_ids, pos0, T, b, /*touches_cache=*/h0 + nh > 24)) return rc;
     DeviceGuard guard(c.cfg.device);
-    cudaError_t e = kata::launch_prep(c, b, T, d_qfull, d_kproj, d_vproj, act_dtype, d_qnorm, d_knorm, (__half*)d_q16, d_q32, d_gate, h0, nh, (cudaStream_t)stream);
+    cudaError_t e = kata::launch_prep(c, b, T, d_qfull, d_kproj, d_vproj, act_dtype, d_qnorm, d_knorm, (__half*)d_q16, d_q32, d_gate, h0, nh, (cudaStream_t)stream, d_axis_pos, axes);
     if (e == cudaSuccess && h0 + nh > 24) { c.wrote_no_rows(); for (int i = 0; i < n; i++) c.wrote_rows_from(b.seq[i], b.pos[i]); }
     else if (e == cudaSuccess) c.wrote_no_rows();
     return e == cudaSuccess ? KATA_OK : cuda_fail(c, e, "prep launch");
+}
+
+int kata_attn_prep(kata_attn_ctx* h, int32_t layer, int32_t n, const int32_t* seq_ids, const int32_t* pos0, int32_t T,
+                   const void* d_qfull, const void* d_kproj, const void* d_vproj, int32_t act_dtype,
+                   const float* d_qnorm, const float* d_knorm, void* d_q16, float* d_q32, float* d_gate, int32_t h0, int32_t nh, void* stream) {
+    if (!h) return KATA_ERR_ARG;
+    return prep_call(h, layer, n, seq_ids, pos0, T, nullptr, 0, d_qfull, d_kproj, d_vproj, act_dtype, d_qnorm, d_knorm, d_q16, d_q32, d_gate, h0, nh, stream);
+}
+
+int kata_attn_prep_axes(kata_attn_ctx* h, int32_t layer, int32_t n, const int32_t* seq_ids, const int32_t* pos0, int32_t T, const int32_t* d_axis_pos, const int32_t* section, int32_t interleaved,
+                        const void* d_qfull, const void* d_kproj, const void* d_vproj, int32_t act_dtype,
+                        const float* d_qnorm, const float* d_knorm, void* d_q16, float* d_q32, float* d_gate, int32_t h0, int32_t nh, void* stream) {
+    if (!h) return KATA_ERR_ARG;
+    if (!d_axis_pos || !section) return fail(h->c, KATA_ERR_ARG, "prep_axes needs the positions and the sections");
+    int32_t axis[32]; uint64_t axes = 0;
+    if (!kata::rotary_axes(32, section, interleaved, axis)) return fail(h->c, KATA_ERR_ARG, "sections %d, %d, %d do not divide the 32 rotary frequencies%s", section[0], section[1], section[2], interleaved ? " when interleaved" : "");
+    for (int i = 0; i < 32; i++) axes |= (uint64_t)axis[i] << (2 * i);
+    return prep_call(h, layer, n, seq_ids, pos0, T, d_axis_pos, axes, d_qfull, d_kproj, d_vproj, act_dtype, d_qnorm, d_knorm, d_q16, d_q32, d_gate, h0, nh, stream);
 }
 
 int kata_attn_kv_quant(kata_attn_ctx* h, int32_t layer, int32_t seq, const void* d_ks, const void* d_vs, int32_t T, int32_t pos0, void* stream) {

@@ -76,7 +76,19 @@ struct Ctx {
 
 // launchers (defined next to their kernels); each returns a cudaError_t from the launch
 cudaError_t launch_prep(Ctx& c, const Batch& b, int T, const void* qfull, const void* kproj, const void* vproj, int act_dtype,
-                        const float* qnorm, const float* knorm, __half* q16, float* q32, float* gate, int h0, int nh, cudaStream_t s);
+                        const float* qnorm, const float* knorm, __half* q16, float* q32, float* gate, int h0, int nh, cudaStream_t s,
+                        const int32_t* axis_pos = nullptr /* [n][T][3], device */, uint64_t axes = 0 /* two bits per frequency */);
+// The axis of each of n rotary frequencies (kata_attn_prep_axes); false unless every axis gets section[axis] of them.
+inline bool rotary_axes(int n, const int32_t* section, int interleaved, int32_t* axis) {
+    if (section[0] < 0 || section[1] < 0 || section[2] < 0 || (int64_t)section[0] + section[1] + section[2] != n) return false;
+    int32_t count[3] = {0, 0, 0};
+    for (int i = 0; i < n; i++) {
+        const int a = i % 3;
+        axis[i] = interleaved ? ((a && i < 3 * (int64_t)section[a]) ? a : 0) : i < section[0] ? 0 : i < section[0] + section[1] ? 1 : 2;
+        count[axis[i]]++;
+    }
+    return count[0] == section[0] && count[1] == section[1] && count[2] == section[2];
+}
 cudaError_t launch_kv_quant(Ctx& c, int64_t row0, const __half* ks, const __half* vs, int T, cudaStream_t s);
 cudaError_t launch_decode_mma(Ctx& c, const Batch& b, int T, int first_pos, int n_items, const __half* q16, const float* gate, void* out, int out_dtype,
                               float* part_out /* non-null: write merged partials instead of the gated output */, cudaStream_t s);

@@ -16,19 +16,16 @@ namespace kata {
 
 bool make_rot_tab(RotTab& t, int rot_dim, double theta, const int32_t* section, int interleaved) {
     const int n = rot_dim / 2;
-    if (rot_dim < 0 || rot_dim % 2 || n > kPagedMaxRot || section[0] < 0 || section[1] < 0 || section[2] < 0 || (int64_t)section[0] + section[1] + section[2] != n) return false;
+    if (rot_dim < 0 || rot_dim % 2 || n > kPagedMaxRot) return false;
     if (n && !(theta > 0.0 && std::isfinite(theta))) return false;
     t = RotTab{};
-    int count[3] = {0, 0, 0};
+    if (!rotary_axes(n, section, interleaved, t.axis)) return false;
     for (int i = 0; i < n; i++) {
-        const int a = i % 3;
-        t.axis[i] = interleaved ? ((a && i < 3 * section[a]) ? a : 0) : i < section[0] ? 0 : i < section[0] + section[1] ? 1 : 2;
-        count[t.axis[i]]++;
         const long double turns = powl((long double)theta, -(long double)i / n) / 6.283185307179586476925286766559L;
         const long double frac = turns - floorl(turns);
         t.freq[i] = (uint64_t)(int64_t)llrintl((frac >= 0.5L ? frac - 1.0L : frac) * 18446744073709551616.0L);   // modulo one turn
     }
-    return count[0] == section[0] && count[1] == section[1] && count[2] == section[2];
+    return true;
 }
 
 namespace {

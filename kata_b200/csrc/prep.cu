@@ -81,10 +81,11 @@ __device__ __forceinline__ void quant_store_row_g4(const __half (&hv)[8], int8_t
 }
 
 // grid (ceil(nh / 8), T, n) x 256 threads: warp w of a CTA handles head slot h0 + 8*blockIdx.x + w of one token
-template <typename TIn, bool K8, bool V8, bool KG>
+// AXES: each frequency takes its position from one of the token's three (two bits of `axes` per frequency), a load and a product more per row
+template <typename TIn, bool K8, bool V8, bool KG, bool AXES>
 __global__ void __launch_bounds__(256) prep_kernel(const Batch b, const int T, const TIn* __restrict__ qfull, const TIn* __restrict__ kproj, const TIn* __restrict__ vproj,
                                                    const float* __restrict__ qnorm, const float* __restrict__ knorm, __half* __restrict__ q16, float* __restrict__ q32, float* __restrict__ gate,
-                                                   void* k_arena, void* v_arena, __half* ksc, __half* vsc, const int h0, const int nh, const int round_mode, const int kvh_mask) {
+                                                   void* k_arena, void* v_arena, __half* ksc, __half* vsc, const int h0, const int nh, const int round_mode, const int kvh_mask, const int32_t* __restrict__ axis_pos, const uint64_t axes) {
     pdl_wait(); pdl_launch_dependents();   // launched with programmatic stream serialisation
     const int lane = threadIdx.x & 31, slot = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (slot >= nh) return;
@@ -126,7 +127,8 @@ __global__ void __launch_bounds__(256) prep_kernel(const Batch b, const int T, c
 #pragma unroll
     for (int s = 0; s < 8; s++) x[s] = __fmul_rn(__fmul_rn(v[s], r), __ldg(w + 32 * s + lane));
     {   // partial RoPE: pair (lane, lane + 32) = elements 0 and 1 of this lane; the angle is formed in fp32 from the shared table
-        const float theta = __fmul_rn((float)pos, c_inv_freq[lane]);
+        const int p = AXES ? __ldcg(axis_pos + tok * 3 + (int)(axes >> (2 * lane) & 3)) : pos;
+        const float theta = __fmul_rn((float)p, c_inv_freq[lane]);
         float sn, cs; sincosf(theta, &sn, &cs);
         const float a = x[0], bb = x[1];
         x[0] = __fsub_rn(__fmul_rn(a, cs), __fmul_rn(bb, sn)); x[1] = __fadd_rn(__fmul_rn(a, sn), __fmul_rn(bb, cs));
@@ -232,14 +234,16 @@ cudaError_t launch_out_fwht(const float* x, const float* sign, float* out, int64
 }
 
 cudaError_t launch_prep(Ctx& c, const Batch& b, int T, const void* qfull, const void* kproj, const void* vproj, int act_dtype,
-                        const float* qnorm, const float* knorm, __half* q16, float* q32, float* gate, int h0, int nh, cudaStream_t s) {
+                        const float* qnorm, const float* knorm, __half* q16, float* q32, float* gate, int h0, int nh, cudaStream_t s, const int32_t* axis_pos, uint64_t axes) {
     const dim3 grid((nh + 7) / 8, T, b.n), block(256);
     const int mode = c.cfg.kv_mode;
     cudaError_t le = cudaSuccess;
-#define KATA_PREP(TIN, K8, V8) le = mode == KATA_KV_INT8G ? launch_pdl(prep_kernel<TIN, true, true, true>, grid, block, 0, s, b, T, (const TIN*)qfull, (const TIN*)kproj, (const TIN*)vproj, qnorm, knorm, q16, q32, gate, c.k_arena, c.v_arena, c.ksc, c.vsc, h0, nh, (int)c.cfg.quant_round, ((1 << c.kvh_n) - 1) << c.kvh_lo) : launch_pdl(prep_kernel<TIN, K8, V8, false>, grid, block, 0, s, b, T, (const TIN*)qfull, (const TIN*)kproj, (const TIN*)vproj, qnorm, knorm, q16, q32, gate, c.k_arena, c.v_arena, c.ksc, c.vsc, h0, nh, (int)c.cfg.quant_round, ((1 << c.kvh_n) - 1) << c.kvh_lo)
-    if (act_dtype == KATA_ACT_F32) { if (mode == KATA_KV_INT8) KATA_PREP(float, true, true); else if (mode == KATA_KV_INT8V) KATA_PREP(float, false, true); else KATA_PREP(float, false, false); }
-    else if (act_dtype == KATA_ACT_BF16) { if (mode == KATA_KV_INT8) KATA_PREP(__nv_bfloat16, true, true); else if (mode == KATA_KV_INT8V) KATA_PREP(__nv_bfloat16, false, true); else KATA_PREP(__nv_bfloat16, false, false); }
-    else { if (mode == KATA_KV_INT8) KATA_PREP(__half, true, true); else if (mode == KATA_KV_INT8V) KATA_PREP(__half, false, true); else KATA_PREP(__half, false, false); }
+#define KATA_PREP(TIN, K8, V8, KG) le = launch_pdl(axis_pos ? prep_kernel<TIN, K8, V8, KG, true> : prep_kernel<TIN, K8, V8, KG, false>, grid, block, 0, s, b, T, (const TIN*)qfull, (const TIN*)kproj, (const TIN*)vproj, qnorm, knorm, q16, q32, gate, c.k_arena, c.v_arena, c.ksc, c.vsc, h0, nh, (int)c.cfg.quant_round, ((1 << c.kvh_n) - 1) << c.kvh_lo, axis_pos, axes)
+#define KATA_PREP_MODE(TIN) if (mode == KATA_KV_INT8G) KATA_PREP(TIN, true, true, true); else if (mode == KATA_KV_INT8) KATA_PREP(TIN, true, true, false); else if (mode == KATA_KV_INT8V) KATA_PREP(TIN, false, true, false); else KATA_PREP(TIN, false, false, false)
+    if (act_dtype == KATA_ACT_F32) { KATA_PREP_MODE(float); }
+    else if (act_dtype == KATA_ACT_BF16) { KATA_PREP_MODE(__nv_bfloat16); }
+    else { KATA_PREP_MODE(__half); }
+#undef KATA_PREP_MODE
 #undef KATA_PREP
     if (le != cudaSuccess) return le;
     c.launches++;

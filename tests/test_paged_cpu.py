@@ -195,3 +195,7 @@ def test_null_contexts_are_refused(L):
     assert L.kata_paged_fork(None, 0, 1, 1, None) == ARG and L.kata_paged_prep(None, 0, 1, None, None, 1, None, None, None, None, None, 0, None, None, None, None, None) == ARG
     assert L.kata_paged_decode(None, 0, 1, None, None, 1, None, None, None, 0, 0, None) == ARG and L.kata_paged_evict(None, 0, 1, 1, None, None, None, 1, 0, 0, None, None) == ARG
     assert L.kata_paged_import(None, 0, 0, 0, 1, 0, None, 0, 0, 0, None) == ARG and L.kata_paged_last_error(None) == b"null context" and not L.kata_paged_plane_ptr(None, 0, 0)
+
+
+def test_prep_axes_refuses_a_null_context(L):
+    assert L.kata_attn_prep_axes(None, 0, 1, None, None, 1, None, None, 0, None, None, None, 0, None, None, None, None, None, 0, 32, None) == ARG
