@@ -100,7 +100,7 @@ int kata_paged_prep(kata_paged_ctx* ctx, int32_t layer, int32_t n, const int32_t
 
 /* Attention of the T newest tokens of each sequence (1..KATA_MAX_VERIFY) over its n_slots[b] slots: token t sees slots [0, n_slots[b] - T + 1 + t).
  *   d_out [n][T][heads][head_dim] out_dtype = softmax(q k^T) v (* sigmoid(gate) when d_gate is given); a token that sees no slot gets zeros.
- * fp32 outputs carry the probabilities in two fp16 terms into the matrix product (about 22 bits), bf16 and fp16 outputs in one.
+ * The probabilities go into the matrix product in two fp16 terms (about 22 bits); for int8 caches with bf16 or fp16 outputs in one (2^-11 relative).
  * accumulate != 0 (KATA_PAGED_WEIGHTS; each sequence once per call): weight[head][slot] += the slot's probability, summed over the tokens and over the
  * query heads of the KV head. No atomics: the sums come out the same in every run. */
 int kata_paged_decode(kata_paged_ctx* ctx, int32_t layer, int32_t n, const int32_t* seq_ids, const int32_t* n_slots, int32_t T,

@@ -696,15 +696,16 @@ int split_paged_tiles(PagedPlan& p, int tile_keys, int sm_count) {
         // end of a segment moves there: less than what the second piece would cost.
         p.n_ctas = std::max(1, std::min(sm_count, total));
         const int pad = total >= (int64_t)sm_count * 4 * kPad ? kPad : 0, snap = pad ? kSnap : 0; const int64_t places = total + (int64_t)n_seg * pad;
-        int c = 0; int64_t place = 0;   // of the segment: its pad, then its tiles
+        int c = 0; int64_t place = 0, next = 0;   // place: of the segment (its pad, then its tiles); next: of cut c
         for (int i = 0; i < p.n; i++) {
             const int nt = plan_ntiles(p, i);
             for (int kv = 0; kv < p.kv_heads; kv++, place += nt + pad) {
                 int cuts_inside = 0;
-                for (; c < p.n_ctas && places * c / p.n_ctas < place + nt + pad; c++) {
-                    int in = (int)(places * c / p.n_ctas - place) - pad;
+                while (c < p.n_ctas && next < place + nt + pad) {
+                    int in = (int)(next - place) - pad;
                     in = in <= snap ? 0 : in >= nt - snap ? nt : in;
                     p.cut[c] = p.tile_start[i] + kv * nt + in; cuts_inside += in > 0 && in < nt;
+                    next = places * ++c / p.n_ctas;
                 }
                 most = std::max(most, cuts_inside + 1);
             }

@@ -5,6 +5,7 @@ Tolerances are those of the arithmetic: half a step of the output type (2^-11 fp
 (an error of a score of at most 32 * 2^-23 of the sum of its terms' magnitudes: 16 chained matrix instructions of 16 terms), probabilities rounded to
 fp16 for 16-bit outputs (2^-11), int8 codes carried with a bias of 1152 for those."""
 import math
+import random
 
 import pytest
 import torch
@@ -174,6 +175,87 @@ def test_decode_of_a_full_batch_and_the_same_sequence_twice(capi):
     assert (two[:2] - got[[100, 7]]).abs().max() < 1e-5
     ref, _, mag = _attend(ctx, 0, 100, 3, 1, q16[100])
     _check_out(ctx, two[2].view(1, 4, 128), ref, q16[100], mag, 3, torch.float32)
+    ctx.close()
+
+
+@pytest.mark.parametrize("layout", [(24, 4, 256), (32, 8, 128)])
+@pytest.mark.parametrize("kv,T,out", [("fp16", 1, torch.bfloat16), ("fp16", 2, torch.float32), ("int8", 1, torch.float32), ("int8", 1, torch.bfloat16), ("int8", 3, torch.float16)])
+@pytest.mark.parametrize("order", ["mixed", "rising"])
+def test_ragged_batches_pass_from_segment_to_segment(capi, layout, kv, T, out, order):
+    """CTAs that work on many short segments, on parts of long ones and on whole ones in one launch; the weights of the same pass; the same bits again."""
+    H, KH, D = layout
+    r = random.Random(T * 7 + KH)
+    slots = [0, 1, 7900, 17] + [r.choice([r.randint(1, 200), r.randint(200, 3000), r.randint(3000, 9000)]) for _ in range(36)]
+    slots = sorted(slots) if order == "rising" else slots
+    g = _gen(sum(slots))
+    ctx = _context(capi, slots, layout, 32, kv, fill=g, weights=True)
+    if kv == "fp16":
+        for s, n in enumerate(slots):
+            rows = _rows(ctx, s, len(ctx.pages(s)) * 32)[n:]
+            for p in ("k", "v"):
+                ctx.plane(0, p).view(-1, KH, D)[rows] = float("nan")
+    q16 = (_randn(g, len(slots), T, H * D) / math.sqrt(D)).half()
+    got = ctx.decode(0, range(len(slots)), slots, T, q16, out_dtype=out, accumulate=True)
+    assert torch.equal(got, ctx.decode(0, range(len(slots)), slots, T, q16, out_dtype=out))
+    ctx.check()
+    for s, n in enumerate(slots):
+        ref, w, mag = _attend(ctx, 0, s, n, T, q16[s])
+        if n:
+            _check_out(ctx, got[s].view(T, H, D), ref, q16[s], mag, n, out)
+            tol = 2 * _score_error(ctx, q16[s], mag, True) + 2.0 ** -20
+            assert (_per_head(ctx, 0, "weight", s, n).to(F8) - w).abs().le(tol * w + 2.0 ** -24).all()
+        else:
+            assert (got[s] == 0).all()
+    ctx.close()
+
+
+@pytest.mark.parametrize("D,kv", [(256, "fp16"), (256, "int8"), (128, "fp16"), (128, "int8")])
+def test_decode_at_the_limits_of_heads_and_batch(capi, D, kv):
+    """16 query heads on each of 16 KV heads, 256 sequences."""
+    g = _gen(D)
+    slots = [r % 41 for r in range(256)]
+    ctx = _context(capi, slots, (256, 16, D), 16, kv, fill=g, weights=True)
+    q16 = (_randn(g, 256, 2, 256 * D) / math.sqrt(D)).half()
+    got = ctx.decode(0, range(256), slots, 2, q16, accumulate=True).view(256, 2, 256, D)
+    ctx.check()
+    for s in (0, 1, 2, 40, 128, 255):
+        n = slots[s]
+        ref, w, mag = _attend(ctx, 0, s, n, 2, q16[s])
+        if n:
+            _check_out(ctx, got[s], ref, q16[s], mag, n, torch.float32)
+            tol = 2 * _score_error(ctx, q16[s], mag, True) + 2.0 ** -20
+            assert (_per_head(ctx, 0, "weight", s, n).to(F8) - w).abs().le(tol * w + 2.0 ** -23).all()   # (two passes: a second sum)
+        else:
+            assert (got[s] == 0).all()
+    ctx.close()
+
+
+def test_two_graphs_of_one_context_replayed_in_turn(capi):
+    """Graphs share the context's scratch; on one stream, one behind the other, each leaves it as the other needs it."""
+    g = _gen(11)
+    slots = [5000, 40, 2500, 0, 700]
+    ctx = _context(capi, slots, fill=g, weights=True)
+    q16 = (_randn(g, 5, 2, 6144) / 16).half()
+    q = [q16, q16[2:4].contiguous()]
+    ids, held = [list(range(5)), [2, 3]], [slots, [2400, 0]]
+    want = [ctx.decode(0, ids[i], held[i], 2, q[i]) for i in range(2)]
+    base = [(ctx.plane(0, "weight").zero_(), ctx.decode(0, ids[i], held[i], 2, q[i], accumulate=True), ctx.plane(0, "weight").clone())[2] for i in range(2)]
+    ctx.plane(0, "weight").zero_()
+    outs, graphs, s = [torch.zeros_like(x) for x in want], [], torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for i in range(2):
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr, stream=s):
+                ctx.decode(0, ids[i], held[i], 2, q[i], out=outs[i], accumulate=True)
+            graphs.append(gr)
+        for i in (0, 1, 1, 0):
+            graphs[i].replay()
+    torch.cuda.synchronize()
+    ctx.check()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    w = 2 * (base[0].to(F8) + base[1].to(F8))
+    assert (ctx.plane(0, "weight").to(F8) - w).abs().le(4 * 2.0 ** -24 * w).all()   # four sums, rounded
     ctx.close()
 
 
