@@ -118,7 +118,7 @@ int kata_paged_evict(kata_paged_ctx* ctx, int32_t layer, int32_t n_layers, int32
  * that kata_attn_prefill has worked on goes on in pages. Same kv_mode, 24 heads, 4 KV heads, head_dim 256, same device. Weights start at 0, ages at age0. */
 int kata_paged_import(kata_paged_ctx* ctx, int32_t layer, int32_t seq, int32_t slot0, int32_t n_rows, int32_t age0, kata_attn_ctx* src, int32_t src_layer, int32_t src_seq, int32_t src_pos, void* stream);
 
-/* How a decode launch would be shared out (host only, no GPU): tile_keys keys per tile, the tiles of all (sequence, KV head) segments in one list, CTA c works on tiles
+/* How a decode launch would be shared out (host only, no GPU): tile_keys (16, 32 or 64) keys per tile, the tiles of all (sequence, KV head) segments in one list, CTA c works on tiles
  * [first_tile[c], first_tile[c + 1]). Returns the number of CTAs, -1 for arguments out of range; *max_contrib: CTAs of the most-cut segment. */
 int kata_paged_decode_plan(int32_t n, const int32_t* n_keys, int32_t kv_heads, int32_t tile_keys, int32_t sm_count, int32_t* first_tile, int32_t first_tile_cap, int32_t* max_contrib);
 

@@ -89,8 +89,7 @@ int kata_paged_create(const kata_paged_config* cfg, kata_paged_ctx** out) {
     c.width = c.pages->width;
     DeviceGuard guard(cfg->device);
     cudaDeviceGetAttribute(&c.sm_count, cudaDevAttrMultiProcessorCount, cfg->device);
-    const int tile = kata::paged_tile_keys(c);
-    c.box_groups = (tile == 32 && cfg->page_size >= 32) ? 2 : 1;
+    c.box_groups = ((hd == 128 || c.int8()) && cfg->page_size >= 32) ? 2 : 1;   // tiles of 32 slots and more
     bool ok = true;
     for (int p = 0; p < KATA_PAGED_PLANES && ok; p++) {
         const size_t bytes = (size_t)rows * c.plane_row_bytes(p);
@@ -105,9 +104,8 @@ int kata_paged_create(const kata_paged_config* cfg, kata_paged_ctx** out) {
     alloc(&c.part_o, kata::paged_part_floats(c) * 4, false); alloc(&c.part_ml, kata::paged_part_ml_floats(c) * 4, false);
     alloc(&c.counters, (size_t)KATA_PAGED_MAX_BATCH * KVH * 4, true); alloc(&c.d_err, 4, true);
     if (c.weights()) {
-        c.score_tiles = (int64_t)KVH * ((int64_t)cfg->n_pages * std::max(1, cfg->page_size / tile) + KATA_PAGED_MAX_BATCH);   // no page is shared, so the pool bounds a launch's tiles
         const int per_pass = std::max(1, 16 / c.group) * c.group;
-        alloc(&c.scores, (size_t)c.score_tiles * tile * (std::min(per_pass, KATA_MAX_VERIFY * c.group) <= 8 ? 8 : 16) * 4, false);
+        alloc(&c.scores, (size_t)kata::paged_score_slots(c) * (std::min(per_pass, KATA_MAX_VERIFY * c.group) <= 8 ? 8 : 16) * 4, false);
         alloc(&c.fin_ml, (size_t)KATA_PAGED_MAX_BATCH * KVH * 16 * 2 * 4, false);
     }
     if (!ok) { cudaGetLastError(); kata_paged_destroy(h); return KATA_ERR_NOMEM; }

@@ -3,7 +3,7 @@
 // With weights: w[kv head][j] += sum_r p_rj / l_r, which needs the joined (m, l); the fp32 scores are kept and a second, small kernel forms the sums.
 //
 // Bound by HBM (4096 bytes of K+V per slot at fp16 with 4 heads of 256, each read once), so the work split is that of the contiguous decode kernel:
-// the tiles (16 or 32 slots of one KV head, 16 KiB of K+V) of all (sequence, KV head) segments form one list, cut into one contiguous range per SM, the
+// the tiles (16, 32 or 64 slots of one KV head, 16 KiB of K+V) of all (sequence, KV head) segments form one list, cut into one contiguous range per SM, the
 // ranges' partial rows joined by the last CTA of a segment (at most 8 of them) or by a combine grid. Inside a CTA four rings of a score warp and two value warps take
 // the tiles in turn; producer warps refill the rings' stages with TMA. The three kinds of warps pass from one segment into the next on their own (mbarriers for what they hand over, named barriers
 // within a kind): the producers and the score warps work on the next segment while the value warps add the rings up and write the rows. With all of them stopping at a segment's end, 32 int8
@@ -45,7 +45,7 @@ constexpr int kOffEBars = kRings * kMaxStages * 8, kOffPBars = 2 * kOffEBars, kO
 template <int HD, bool K8, int NR> struct PGeo {   // NR: column tiles of 8 query rows
     static constexpr int kThreads = (3 * kRings + (K8 ? kRings : 1)) * 32;               // fp16: one producer warp, lane r for ring r (in step: 121 us for 37 sequences of 5,200 slots, 127 with one per ring, 140 with one whose lanes drift apart); int8: one per ring
     static constexpr int kRowBytes = HD * (K8 ? 1 : 2);                                  // bytes of a head row
-    static constexpr int kNK = (HD == 256 && !K8) ? 1 : 2, kTile = 16 * kNK;             // 16-slot groups and slots per tile
+    static constexpr int kNK = (HD == 256 && !K8) ? 1 : (HD == 128 && K8 && NR == 1) ? 4 : 2, kTile = 16 * kNK;   // 16-slot groups and slots per tile: 16 KiB of K and V (8 with 8 heads' worth of int8 rows of 128: P's slots have no more room)
     static constexpr int kGroupBytes = 16 * kRowBytes, kHalfBytes = kNK * kGroupBytes;   // K (or V) of one group, of one tile
     static constexpr int kStageBytes = 2 * kHalfBytes, kStages = kStageBytes == 16384 ? 3 : 6;
     static constexpr int kRingBytes = kStages * kStageBytes;
@@ -56,7 +56,7 @@ template <int HD, bool K8, int NR> struct PGeo {   // NR: column tiles of 8 quer
     // NR = 1: a block of its own, and two slots for the rings' (m, l): the score warps go on into the next segment. NR = 2: no room, it lies where the P slots are and the score warps wait.
     static constexpr int kSums = NR == 1 ? 2 : 1;
     static constexpr int kOffBars = kQBytes, kOffMl = kOffBars + kBarBytes, kOffPair = kOffMl + kSums * 512 + 128, kOffRed = kOffPair + (NR == 1 ? kRings * 2 * kPBytes : 0);
-    static constexpr int kOffScale = NR == 1 ? kOffRed + kRedBytes : kOffPair + (kRings * 2 * kPBytes > kRedBytes ? kRings * 2 * kPBytes : kRedBytes), kOffStages = kOffScale + (K8 ? kRings * kStages * 128 : 0);   // scales: [ring][stage][32 slots] K and V packed
+    static constexpr int kOffScale = NR == 1 ? kOffRed + kRedBytes : kOffPair + (kRings * 2 * kPBytes > kRedBytes ? kRings * 2 * kPBytes : kRedBytes), kOffStages = kOffScale + (K8 ? kRings * kStages * kTile * 4 : 0);   // scales: [ring][stage][slot] K and V packed
     static constexpr int kSmem = kOffStages + 1024 + kRings * kRingBytes;
     static_assert(kSmem <= 232448, "shared memory");
 };
@@ -189,9 +189,11 @@ __device__ __forceinline__ void paged_publish(const uint32_t p_sm, float* alpha,
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[x]));
             lo[x] = pack_h2(u - f.x, v - f.y);
         }
-        const uint32_t at = p_sm + (nr * 8 + (lane & 7)) * G::kPStride + ((lane >> 3) & (2 * NK - 1)) * 16;
-        if constexpr (NK == 2) { stsm_x4_t(at, hi[0], hi[1], hi[2], hi[3]); if (two_terms) stsm_x4_t(at + G::kPTerm, lo[0], lo[1], lo[2], lo[3]); }
-        else { stsm_x2_t(at, hi[0], hi[1]); if (two_terms) stsm_x2_t(at + G::kPTerm, lo[0], lo[1]); }
+        const uint32_t at = p_sm + (nr * 8 + (lane & 7)) * G::kPStride + ((lane >> 3) & (NK == 1 ? 1 : 3)) * 16;
+        if constexpr (NK > 1) {
+#pragma unroll
+            for (int x = 0; x < 2 * NK; x += 4) { stsm_x4_t(at + x * 16, hi[x], hi[x + 1], hi[x + 2], hi[x + 3]); if (two_terms) stsm_x4_t(at + x * 16 + G::kPTerm, lo[x], lo[x + 1], lo[x + 2], lo[x + 3]); }
+        } else { stsm_x2_t(at, hi[0], hi[1]); if (two_terms) stsm_x2_t(at + G::kPTerm, lo[0], lo[1]); }
         if (lane < 4) *reinterpret_cast<float2*>(alpha + nr * 8 + 2 * lane) = make_float2(al[nr][0], al[nr][1]);
     }
 }
@@ -213,9 +215,12 @@ __device__ __forceinline__ void paged_values(const uint32_t v_sm, const uint32_t
 #pragma unroll
     for (int nr = 0; nr < NR; nr++) {
         al[nr] = *reinterpret_cast<const float2*>(alpha + nr * 8 + 2 * (lane & 3));
-        const uint32_t at = p_sm + (nr * 8 + (lane & 7)) * G::kPStride + ((lane >> 3) & (2 * NK - 1)) * 16;
+        const uint32_t at = p_sm + (nr * 8 + (lane & 7)) * G::kPStride + ((lane >> 3) & (NK == 1 ? 1 : 3)) * 16;
         auto load = [&](uint32_t a, uint32_t (&x)[2 * NK]) {
-            if constexpr (NK == 2) ldsm_x4(a, x[0], x[1], x[2], x[3]);
+            if constexpr (NK > 1) {
+#pragma unroll
+                for (int y = 0; y < 2 * NK; y += 4) ldsm_x4(a + y * 16, x[y], x[y + 1], x[y + 2], x[y + 3]);
+            }
             else asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(a));
         };
         load(at, ph[nr]);
@@ -317,6 +322,7 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
         // ahead. int8: lane j also fetches the K and V scale of slot j, three tiles ahead (under load a request takes as long as all that is in flight before it), the page number of
         // that three tiles earlier still, and stores it before the tile's copy is issued. Unrolled by three so that every load has registers of its own. What the first three tiles of the next
         // segment need is requested during this one (148 int8 sequences of 3,600 slots, four segments per CTA: 203 us without).
+        constexpr int SL = K8 ? kTile / 32 : 1;   // scales per lane: slots lane, lane + 32
         struct Seg { int kvh, lt0, n_here, n_mine, last; const int32_t* table; };
         auto segment = [&](int first) {
             while (p.tile_start[b + 1] <= first) b++;
@@ -324,23 +330,29 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
             return Seg{kvh, lt0, n_here, n_here > ring ? (n_here - ring + kRings - 1) / kRings : 0, max(p.kend[b] - 1, 0), tables + (int64_t)p.seq[b] * p.width};
         };
         auto first_slot = [&](const Seg& g, int i) { return (g.lt0 + ring + i * kRings) * kTile; };
-        auto load_pages = [&](const Seg& g, int i, int32_t (&x)[2]) {
-            x[0] = __ldcg(g.table + (min(first_slot(g, i), g.last) >> p.page_shift));
-            x[1] = p.groups_per_box < NK ? __ldcg(g.table + (min(first_slot(g, i) + 16, g.last) >> p.page_shift)) : 0;
+        auto load_pages = [&](const Seg& g, int i, int32_t (&x)[NK]) {   // of every box
+#pragma unroll
+            for (int y = 0; y < NK; y++) if (!(y & (p.groups_per_box - 1))) x[y] = __ldcg(g.table + (min(first_slot(g, i) + 16 * y, g.last) >> p.page_shift));
         };
-        auto scale_slot = [&](const Seg& g, int i) { return min(first_slot(g, i) + lane, g.last); };   // slots behind the last repeat it: finite scales, and probabilities 0
-        auto scale_page = [&](const Seg& g, int i) { return __ldcg(g.table + (scale_slot(g, i) >> p.page_shift)); };
-        auto load_scales = [&](const Seg& g, int i, int32_t page, unsigned short (&x)[2]) {
-            const int64_t at = (((int64_t)page << p.page_shift) + (scale_slot(g, i) & mask)) * kvh_n + g.kvh;   // ksc, vsc: this layer's planes
-            x[0] = __ldcg(reinterpret_cast<const unsigned short*>(ksc) + at); x[1] = __ldcg(reinterpret_cast<const unsigned short*>(vsc) + at);
+        auto scale_slot = [&](const Seg& g, int i, int x) { return min(first_slot(g, i) + 32 * x + lane, g.last); };   // slots behind the last repeat it: finite scales, and probabilities 0
+        auto scale_pages = [&](const Seg& g, int i, int32_t (&page)[SL]) {
+#pragma unroll
+            for (int x = 0; x < SL; x++) page[x] = __ldcg(g.table + (scale_slot(g, i, x) >> p.page_shift));
         };
-        Seg sg = segment(tile), next = sg; int32_t pg[3][2], npg[3][2], spg[3], nspg[3]; unsigned short sc8[3][2], nsc8[3][2];
+        auto load_scales = [&](const Seg& g, int i, const int32_t (&page)[SL], unsigned short (&sc)[SL][2]) {
+#pragma unroll
+            for (int x = 0; x < SL; x++) {
+                const int64_t at = (((int64_t)page[x] << p.page_shift) + (scale_slot(g, i, x) & mask)) * kvh_n + g.kvh;   // ksc, vsc: this layer's planes
+                sc[x][0] = __ldcg(reinterpret_cast<const unsigned short*>(ksc) + at); sc[x][1] = __ldcg(reinterpret_cast<const unsigned short*>(vsc) + at);
+            }
+        };
+        Seg sg = segment(tile), next = sg; int32_t pg[3][NK], npg[3][NK], spg[3][SL], nspg[3][SL]; unsigned short sc8[3][SL][2], nsc8[3][SL][2];
         if (issues) { load_pages(sg, 0, pg[0]); load_pages(sg, 1, pg[1]); load_pages(sg, 2, pg[2]); }
         if (K8) {
 #pragma unroll
-            for (int j = 0; j < 3; j++) spg[j] = scale_page(sg, j);
+            for (int j = 0; j < 3; j++) scale_pages(sg, j, spg[j]);
 #pragma unroll
-            for (int j = 0; j < 3; j++) { load_scales(sg, j, spg[j], sc8[j]); spg[j] = scale_page(sg, j + 3); }
+            for (int j = 0; j < 3; j++) { load_scales(sg, j, spg[j], sc8[j]); scale_pages(sg, j + 3, spg[j]); }
         }
         while (true) {
             tile += sg.n_here;
@@ -348,12 +360,12 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
             if (more) {
                 next = segment(tile);
                 if (issues) { load_pages(next, 0, npg[0]); load_pages(next, 1, npg[1]); load_pages(next, 2, npg[2]); }
-                if (K8) { nspg[0] = scale_page(next, 0); nspg[1] = scale_page(next, 1); nspg[2] = scale_page(next, 2); }
+                if (K8) { scale_pages(next, 0, nspg[0]); scale_pages(next, 1, nspg[1]); scale_pages(next, 2, nspg[2]); }
             }
             const int n_steps = K8 ? sg.n_mine : (sg.n_here + kRings - 1) / kRings;   // the same for all lanes: they stay in step
             auto next_scales = [&]() {
 #pragma unroll
-                for (int j = 0; j < 3; j++) { load_scales(next, j, nspg[j], nsc8[j]); nspg[j] = scale_page(next, j + 3); }
+                for (int j = 0; j < 3; j++) { load_scales(next, j, nspg[j], nsc8[j]); scale_pages(next, j + 3, nspg[j]); }
             };
             if (K8 && more && n_steps <= 3) next_scales();
             for (int i0 = 0; i0 < n_steps; i0 += 3) {
@@ -367,20 +379,21 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
                     if (has && !dead && !mbar_wait_bounded(ebars + sx * 8, ((cur / kStages) + 1u) & 1u, err)) { dead = true; atomicExch(err, 3); }   // the first time round the wait is for the phase before the first: over at once
                     __syncwarp();
                     if (K8) {
-                        reinterpret_cast<uint32_t*>(smem + G::kOffScale)[(ring * kStages + sx) * 32 + lane] = (uint32_t)sc8[j][0] | (uint32_t)sc8[j][1] << 16;
+#pragma unroll
+                        for (int x = 0; x < SL; x++) reinterpret_cast<uint32_t*>(smem + G::kOffScale)[(ring * kStages + sx) * kTile + 32 * x + lane] = (uint32_t)sc8[j][x][0] | (uint32_t)sc8[j][x][1] << 16;
                         __syncwarp();   // the arrival below publishes them
                     }
                     if (has) {
                         mbar_arrive_expect_tx(bar, (uint32_t)G::kStageBytes);
 #pragma unroll
                         for (int x = 0; x < NK; x++) {
-                            if (x && p.groups_per_box == NK) break;
+                            if (x & (p.groups_per_box - 1)) continue;
                             const int grp = (int)((p.layer_row0 + ((int64_t)pg[j][x] << p.page_shift) + ((first_slot(sg, i) + 16 * x) & mask)) >> 4);
                             tma_load_5d(dst + x * G::kGroupBytes, &tm_k, 0, 0, 0, grp, sg.kvh, bar); tma_load_5d(dst + G::kHalfBytes + x * G::kGroupBytes, &tm_v, 0, 0, 0, grp, sg.kvh, bar);
                         }
                         load_pages(sg, i + 3, pg[j]);   // behind the ring's last tile: the last page again
                     }
-                    if (K8) { load_scales(sg, i + 3, spg[j], sc8[j]); spg[j] = scale_page(sg, i + 6); }
+                    if (K8) { load_scales(sg, i + 3, spg[j], sc8[j]); scale_pages(sg, i + 6, spg[j]); }
                 }
             }
             __syncwarp();
@@ -388,8 +401,10 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
             it += (uint32_t)sg.n_mine; sg = next;
 #pragma unroll
             for (int j = 0; j < 3; j++) {
-                pg[j][0] = npg[j][0]; pg[j][1] = npg[j][1];
-                if (K8) { spg[j] = nspg[j]; sc8[j][0] = nsc8[j][0]; sc8[j][1] = nsc8[j][1]; }
+#pragma unroll
+                for (int x = 0; x < NK; x++) pg[j][x] = npg[j][x];
+#pragma unroll
+                for (int x = 0; x < SL; x++) if (K8) { spg[j][x] = nspg[j][x]; sc8[j][x][0] = nsc8[j][x][0]; sc8[j][x][1] = nsc8[j][x][1]; }
             }
         }
         return;
@@ -437,7 +452,7 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
                 for (int sb = 0; sb < NK; sb++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        if (K8) sc[sb][e] = *reinterpret_cast<const uint32_t*>(smem + G::kOffScale + (ring * kStages + stg) * 128 + (16 * sb + 8 * e + g) * 4);
+                        if (K8) sc[sb][e] = *reinterpret_cast<const uint32_t*>(smem + G::kOffScale + (ring * kStages + stg) * kTile * 4 + (16 * sb + 8 * e + g) * 4);
                         ks[sb][e] = K8 ? __half2float(__ushort_as_half((unsigned short)sc[sb][e])) : 1.0f;
                     }
                 float s[NK][NR][4], al[NR][2];
@@ -718,7 +733,8 @@ int split_paged_tiles(PagedPlan& p, int tile_keys, int sm_count) {
 
 }  // namespace
 
-int paged_tile_keys(const PagedCtx& c) { return (c.cfg.head_dim == 256 && !c.int8()) ? 16 : 32; }
+static int tile_keys_of(const PagedCtx& c, int rows) { return c.cfg.head_dim == 256 ? (c.int8() ? 32 : 16) : (c.int8() && rows <= 8) ? 64 : 32; }   // PGeo::kTile
+int64_t paged_score_slots(const PagedCtx& c) { return (int64_t)c.cfg.kv_heads * ((int64_t)c.cfg.n_pages * c.cfg.page_size + 64 * KATA_PAGED_MAX_BATCH); }   // no page is shared, so the pool bounds a launch's slots; each sequence's are rounded up to a tile
 // (CTA + segment) slots of partial rows
 size_t paged_part_floats(const PagedCtx& c) { return (size_t)(c.sm_count + KATA_PAGED_MAX_BATCH * c.cfg.kv_heads) * 16 * c.cfg.head_dim; }
 size_t paged_part_ml_floats(const PagedCtx& c) { return (size_t)(c.sm_count + KATA_PAGED_MAX_BATCH * c.cfg.kv_heads) * 32; }
@@ -734,15 +750,16 @@ cudaError_t configure_paged_decode(const PagedCtx& c) {   // shared-memory opt-i
 }
 
 cudaError_t launch_paged_decode(PagedCtx& c, int layer, int n, const int32_t* seq, const int32_t* n_slots, int T, const __half* q16, const float* gate, void* out, int out_dtype, bool accumulate, cudaStream_t s) {
-    const int per_pass = std::max(1, 16 / c.group), tile_keys = paged_tile_keys(c), hd = c.cfg.head_dim;
+    const int per_pass = std::max(1, 16 / c.group), hd = c.cfg.head_dim;
     for (int t0 = 0; t0 < T; t0 += per_pass) {   // each pass is independent: all rows are in the cache, token t of the call sees slots below n_slots - T + 1 + t
         PagedPlan p{}; p.n = n; p.T = std::min(per_pass, T - t0); p.group = c.group; p.kv_heads = c.cfg.kv_heads; p.tok_stride = T; p.tok0 = t0;
         p.two_terms = !c.int8() || out_dtype == KATA_ACT_F32; p.page_shift = c.page_shift; p.width = c.width; p.groups_per_box = c.box_groups; p.layer_row0 = (int64_t)layer * c.rows_per_layer;
         for (int i = 0; i < n; i++) { p.seq[i] = seq[i]; p.kend[i] = std::max(0, n_slots[i] - T + t0 + p.T); }
+        const int tile_keys = tile_keys_of(c, c.group * p.T);
         split_paged_tiles(p, tile_keys, c.sm_count);
         // a pass's limits are kend - p.T + 1 + t: where kend was raised to 0 they are 0 or less, as they should be
         const PagedOut o{gate, out, out_dtype, accumulate ? c.fin_ml : nullptr}; float* scores = accumulate ? c.scores : nullptr;
-        if (accumulate && p.tile_start[n] > c.score_tiles) return cudaErrorInvalidValue;   // cannot be: the pool bounds the tiles
+        if (accumulate && (int64_t)p.tile_start[n] * tile_keys > paged_score_slots(c)) return cudaErrorInvalidValue;   // cannot be: the pool bounds them
         cudaError_t e = cudaErrorInvalidValue;
 #define X(HD, K8, NR) if (hd == HD && c.int8() == K8 && (c.group * p.T > 8) == (NR == 2)) e = launch_pdl(paged_decode_kernel<HD, K8, NR>, dim3(p.n_ctas), dim3(PGeo<HD, K8, NR>::kThreads), PGeo<HD, K8, NR>::kSmem, s, c.tm_k, c.tm_v, p, (const int32_t*)c.d_table, q16, o, \
             (const __half*)c.layer_plane(KATA_PAGED_K_SCALE, layer), (const __half*)c.layer_plane(KATA_PAGED_V_SCALE, layer), scores, c.part_o, c.part_ml, c.counters, c.d_err);
@@ -759,7 +776,7 @@ cudaError_t launch_paged_decode(PagedCtx& c, int layer, int n, const int32_t* se
         if (accumulate) {
             const int64_t keys = (int64_t)p.tile_start[n] * tile_keys;
             e = launch_pdl(c.group * p.T > 8 ? paged_weight_kernel<16> : paged_weight_kernel<8>, dim3((unsigned)((keys + 255) / 256)), dim3(256), 0, s, p, (const int32_t*)c.d_table, (const float*)c.scores, (const float*)c.fin_ml,
-                           (float*)c.layer_plane(KATA_PAGED_WEIGHT, layer), tile_keys == 16 ? 4 : 5, c.int8() ? (float)PGeo<256, true, 1>::kPShift : (float)PGeo<256, false, 1>::kPShift);
+                           (float*)c.layer_plane(KATA_PAGED_WEIGHT, layer), tile_keys == 16 ? 4 : tile_keys == 32 ? 5 : 6, c.int8() ? (float)PGeo<256, true, 1>::kPShift : (float)PGeo<256, false, 1>::kPShift);
             if (e != cudaSuccess) return e;
             c.launches++;
         }
@@ -771,7 +788,7 @@ cudaError_t launch_paged_decode(PagedCtx& c, int layer, int n, const int32_t* se
 
 extern "C" int kata_paged_decode_plan(int32_t n, const int32_t* n_keys, int32_t kv_heads, int32_t tile_keys, int32_t sm_count, int32_t* first_tile, int32_t first_tile_cap, int32_t* max_contrib) {
     using namespace kata;
-    if (n < 1 || n > KATA_PAGED_MAX_BATCH || !n_keys || kv_heads < 1 || kv_heads > KATA_PAGED_MAX_KV_HEADS || (tile_keys != 16 && tile_keys != 32) || sm_count < 1 || !first_tile || !max_contrib) return -1;
+    if (n < 1 || n > KATA_PAGED_MAX_BATCH || !n_keys || kv_heads < 1 || kv_heads > KATA_PAGED_MAX_KV_HEADS || (tile_keys != 16 && tile_keys != 32 && tile_keys != 64) || sm_count < 1 || !first_tile || !max_contrib) return -1;
     PagedPlan p{}; p.n = n; p.kv_heads = kv_heads;
     for (int i = 0; i < n; i++) { if (n_keys[i] < 0 || n_keys[i] > KATA_PAGED_MAX_SLOTS) return -1; p.kend[i] = n_keys[i]; }
     *max_contrib = split_paged_tiles(p, tile_keys, sm_count);

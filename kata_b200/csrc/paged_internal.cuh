@@ -23,7 +23,7 @@ struct PagedCtx {
     RotTab* d_rot = nullptr;
     float* part_o = nullptr; float* part_ml = nullptr; int32_t* counters = nullptr; int32_t* d_err = nullptr;   // decode: partial rows of cut segments, their (m, l), tickets
     float* fin_ml = nullptr;              // decode with weights: joined (m, l) of every row of every segment
-    float* scores = nullptr; int64_t score_tiles = 0;   // decode with weights: fp32 scores [tile][key][8 or 16 rows] of one launch; room for so many tiles
+    float* scores = nullptr;   // decode with weights: fp32 scores [tile][key][8 or 16 rows] of one launch
     std::vector<int32_t> stamp; int32_t stamp_now = 0;   // per sequence: the call it was last named in (finds a sequence named twice)
     CUtensorMap tm_k{}, tm_v{}; int box_groups = 1;     // rank-5 tile views of the K and V pools; 16-row groups per box
     int sm_count = 148;
@@ -44,7 +44,7 @@ struct PagedCtx {
 struct PagedBatch { int32_t n; int32_t seq[KATA_PAGED_MAX_BATCH], slot[KATA_PAGED_MAX_BATCH], age[KATA_PAGED_MAX_BATCH]; };
 
 size_t paged_part_floats(const PagedCtx& c); size_t paged_part_ml_floats(const PagedCtx& c);
-int paged_tile_keys(const PagedCtx& c);
+int64_t paged_score_slots(const PagedCtx& c);
 cudaError_t configure_paged_decode(const PagedCtx& c);
 cudaError_t launch_paged_decode(PagedCtx& c, int layer, int n, const int32_t* seq, const int32_t* n_slots, int T, const __half* q16, const float* gate, void* out, int out_dtype, bool accumulate, cudaStream_t s);
 cudaError_t launch_paged_prep(PagedCtx& c, int layer, const PagedBatch& b, int T, const int32_t* axis_pos, const void* q, const void* k, const void* v, int act_dtype,
