@@ -34,7 +34,8 @@ extern "C" {
 #define KATA_PAGED_MAX_GROUP 16      /* query heads per KV head */
 
 enum { KATA_PAGED_GATED = 1,         /* flags: the query rows of kata_paged_prep are [query | gate] per head, as KATA_QFULL_DIM rows are */
-       KATA_PAGED_WEIGHTS = 2 };     /* flags: keep per slot and KV head the attention weight received and the token's age (kata_paged_evict) */
+       KATA_PAGED_WEIGHTS = 2 };     /* flags: keep per slot and KV head the attention weight received and the token's age (kata_paged_evict); takes 32 or 64 bytes more per
+                                      * slot of the pool and KV head for the scores of one launch (64 when a call can have more than 8 query rows per KV head) */
 enum { KATA_PAGED_K = 0, KATA_PAGED_V = 1, KATA_PAGED_K_SCALE = 2, KATA_PAGED_V_SCALE = 3, KATA_PAGED_WEIGHT = 4, KATA_PAGED_AGE = 5, KATA_PAGED_PLANES = 6 };
 
 /* ---- the page table (host only, no GPU): which pages belong to which sequence. A kata_paged context keeps one of its own. Free pages are handed

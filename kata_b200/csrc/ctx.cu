@@ -197,7 +197,7 @@ int kata_attn_prep_axes(kata_attn_ctx* h, int32_t layer, int32_t n, const int32_
                         const void* d_qfull, const void* d_kproj, const void* d_vproj, int32_t act_dtype,
                         const float* d_qnorm, const float* d_knorm, void* d_q16, float* d_q32, float* d_gate, int32_t h0, int32_t nh, void* stream) {
     if (!h) return KATA_ERR_ARG;
-    if (!d_axis_pos || !section) return fail(h->c, KATA_ERR_ARG, "prep_axes needs the positions and the sections");
+    if (!d_axis_pos || !section || ((uintptr_t)d_axis_pos & 3)) return fail(h->c, KATA_ERR_ARG, "prep_axes needs the positions (32-bit integers) and the sections");
     int32_t axis[32]; uint64_t axes = 0;
     if (!kata::rotary_axes(32, section, interleaved, axis)) return fail(h->c, KATA_ERR_ARG, "sections %d, %d, %d do not divide the 32 rotary frequencies%s", section[0], section[1], section[2], interleaved ? " when interleaved" : "");
     for (int i = 0; i < 32; i++) axes |= (uint64_t)axis[i] << (2 * i);

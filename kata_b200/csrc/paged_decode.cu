@@ -45,7 +45,7 @@ constexpr int kOffEBars = kRings * kMaxStages * 8, kOffPBars = 2 * kOffEBars, kO
 template <int HD, bool K8, int NR> struct PGeo {   // NR: column tiles of 8 query rows
     static constexpr int kThreads = (3 * kRings + (K8 ? kRings : 1)) * 32;               // fp16: one producer warp, lane r for ring r (in step: 121 us for 37 sequences of 5,200 slots, 127 with one per ring, 140 with one whose lanes drift apart); int8: one per ring
     static constexpr int kRowBytes = HD * (K8 ? 1 : 2);                                  // bytes of a head row
-    static constexpr int kNK = (HD == 256 && !K8) ? 1 : (HD == 128 && K8 && NR == 1) ? 4 : 2, kTile = 16 * kNK;   // 16-slot groups and slots per tile: 16 KiB of K and V (8 with 8 heads' worth of int8 rows of 128: P's slots have no more room)
+    static constexpr int kNK = (HD == 256 && !K8) ? 1 : (HD == 128 && K8 && NR == 1) ? 4 : 2, kTile = 16 * kNK;   // 16-slot groups and slots per tile: 16 KiB of K and V; 8 KiB for int8 rows of 128 under two column tiles (shared memory has no room for their P). 18 sequences of 15,000 such rows x 8 heads: 95 us, 106 with 8 KiB tiles
     static constexpr int kGroupBytes = 16 * kRowBytes, kHalfBytes = kNK * kGroupBytes;   // K (or V) of one group, of one tile
     static constexpr int kStageBytes = 2 * kHalfBytes, kStages = kStageBytes == 16384 ? 3 : 6;
     static constexpr int kRingBytes = kStages * kStageBytes;
@@ -346,6 +346,7 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
                 sc[x][0] = __ldcg(reinterpret_cast<const unsigned short*>(ksc) + at); sc[x][1] = __ldcg(reinterpret_cast<const unsigned short*>(vsc) + at);
             }
         };
+        uint32_t issued = 0;
         Seg sg = segment(tile), next = sg; int32_t pg[3][NK], npg[3][NK], spg[3][SL], nspg[3][SL]; unsigned short sc8[3][SL][2], nsc8[3][SL][2];
         if (issues) { load_pages(sg, 0, pg[0]); load_pages(sg, 1, pg[1]); load_pages(sg, 2, pg[2]); }
         if (K8) {
@@ -374,9 +375,10 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
                 for (int j = 0; j < 3; j++) {
                     const int i = i0 + j;
                     if (i >= n_steps) break;
-                    const bool has = issues && i < sg.n_mine;
+                    bool has = issues && i < sg.n_mine;
                     const uint32_t cur = it + (uint32_t)i, sx = cur % kStages, bar = bars + sx * 8, dst = ring_stage0 + sx * G::kStageBytes;
                     if (has && !dead && !mbar_wait_bounded(ebars + sx * 8, ((cur / kStages) + 1u) & 1u, err)) { dead = true; atomicExch(err, 3); }   // the first time round the wait is for the phase before the first: over at once
+                    has = has && !dead;   // after a wait that ran out no further copy is asked for
                     __syncwarp();
                     if (K8) {
 #pragma unroll
@@ -384,7 +386,7 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
                         __syncwarp();   // the arrival below publishes them
                     }
                     if (has) {
-                        mbar_arrive_expect_tx(bar, (uint32_t)G::kStageBytes);
+                        mbar_arrive_expect_tx(bar, (uint32_t)G::kStageBytes); issued = cur + 1;
 #pragma unroll
                         for (int x = 0; x < NK; x++) {
                             if (x & (p.groups_per_box - 1)) continue;
@@ -407,6 +409,8 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
                 for (int x = 0; x < SL; x++) if (K8) { spg[j][x] = nspg[j][x]; sc8[j][x][0] = nsc8[j][x][0]; sc8[j][x][1] = nsc8[j][x][1]; }
             }
         }
+        if (issues && *reinterpret_cast<volatile int32_t*>(err) != 0)   // somewhere a wait ran out: its warps no longer wait for copies, so the copies under way are waited for here (within the same limit)
+            for (uint32_t c = issued > (uint32_t)kStages ? issued - kStages : 0; c < issued; c++) mbar_wait_bounded(bars + c % kStages * 8, (c / kStages) & 1u);
         return;
     }
 

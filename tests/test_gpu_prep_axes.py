@@ -136,4 +136,8 @@ def test_refusals(capi):
     with pytest.raises(capi.KataError):   # rows behind the sequence's end
         ctx.prep_axes(0, [0], [7], 2, pos, [32, 0, 0], qf, k, v, qn, kn)
     assert ctx.L.kata_attn_prep_axes(ctx.h, 0, 1, None, None, 2, None, None, 0, None, None, None, 0, None, None, None, None, None, 0, 32, None) == 1
+    import ctypes
+    sec, one = (ctypes.c_int32 * 3)(32, 0, 0), (ctypes.c_int32 * 1)(0)
+    at = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    assert ctx.L.kata_attn_prep_axes(ctx.h, 0, 1, one, one, 2, ctypes.c_void_p(pos.data_ptr() + 2), sec, 0, at(qf), at(k), at(v), 0, at(qn), at(kn), at(qf), None, at(qf), 0, 32, None) == 1   # positions off their boundary: nothing is launched
     ctx.check(); ctx.close()
