@@ -98,15 +98,20 @@ int kata_paged_create(const kata_paged_config* cfg, kata_paged_ctx** out) {
         ok = cudaMalloc(&c.plane[p], bytes) == cudaSuccess;
         if (ok) { c.owned[p] = true; ok = cudaMemset(c.plane[p], 0, bytes) == cudaSuccess; }
     }
-    auto alloc = [&](auto** p, size_t bytes, bool zero) { ok = ok && cudaMalloc((void**)p, bytes) == cudaSuccess && (!zero || cudaMemset(*p, 0, bytes) == cudaSuccess); };
-    alloc(&c.d_table, (size_t)cfg->n_seqs * c.width * 4, true);   // zeros: every entry is a page of the pool at all times
-    alloc(&c.d_rot, sizeof(kata::RotTab), false);
-    alloc(&c.part_o, kata::paged_part_floats(c) * 4, false); alloc(&c.part_ml, kata::paged_part_ml_floats(c) * 4, false);
-    alloc(&c.counters, (size_t)KATA_PAGED_MAX_BATCH * KVH * 4, true); alloc(&c.d_err, 4, true);
-    if (c.weights()) {
-        const int per_pass = std::max(1, 16 / c.group) * c.group;
-        alloc(&c.scores, (size_t)kata::paged_score_slots(c) * (std::min(per_pass, KATA_MAX_VERIFY * c.group) <= 8 ? 8 : 16) * 4, false);
-        alloc(&c.fin_ml, (size_t)KATA_PAGED_MAX_BATCH * KVH * 16 * 2 * 4, false);
+    // the rest in one block (a context in 85 us instead of 126). What has to start at zero lies first (the table's zeros: every entry is a page of the pool at all times)
+    size_t size = 0, zeros = 0;
+    auto part = [&](size_t bytes) { const size_t at = size; size += (bytes + 255) / 256 * 256; return at; };
+    const int per_pass = std::max(1, 16 / c.group) * c.group, score_rows = std::min(per_pass, KATA_MAX_VERIFY * c.group) <= 8 ? 8 : 16;
+    const size_t at_table = part((size_t)cfg->n_seqs * c.width * 4), at_counters = part((size_t)KATA_PAGED_MAX_BATCH * KVH * 4), at_err = part(4);
+    zeros = size;
+    const size_t at_rot = part(sizeof(kata::RotTab)), at_o = part(kata::paged_part_floats(c) * 4), at_ml = part(kata::paged_part_ml_floats(c) * 4);
+    const size_t at_scores = part(c.weights() ? (size_t)kata::paged_score_slots(c) * score_rows * 4 : 0), at_fin = part(c.weights() ? (size_t)KATA_PAGED_MAX_BATCH * KVH * 16 * 2 * 4 : 0);
+    ok = ok && cudaMalloc(&c.block, size) == cudaSuccess && cudaMemset(c.block, 0, zeros) == cudaSuccess;
+    if (ok) {
+        uint8_t* base = (uint8_t*)c.block;
+        c.d_table = (int32_t*)(base + at_table); c.counters = (int32_t*)(base + at_counters); c.d_err = (int32_t*)(base + at_err); c.d_rot = (kata::RotTab*)(base + at_rot);
+        c.part_o = (float*)(base + at_o); c.part_ml = (float*)(base + at_ml);
+        if (c.weights()) { c.scores = (float*)(base + at_scores); c.fin_ml = (float*)(base + at_fin); }
     }
     if (!ok) { cudaGetLastError(); kata_paged_destroy(h); return KATA_ERR_NOMEM; }
     if (cudaMemcpy(c.d_rot, &rot, sizeof rot, cudaMemcpyHostToDevice) != cudaSuccess || kata::configure_paged_decode(c) != cudaSuccess || kata::configure_paged_evict(c) != cudaSuccess ||
@@ -120,8 +125,7 @@ int kata_paged_destroy(kata_paged_ctx* h) {
     if (!h) return KATA_ERR_ARG;
     PagedCtx& c = h->c; DeviceGuard guard(c.cfg.device);
     for (int p = 0; p < KATA_PAGED_PLANES; p++) if (c.owned[p]) cudaFree(c.plane[p]);
-    void* ptrs[] = {c.d_table, c.d_rot, c.part_o, c.part_ml, c.counters, c.d_err, c.scores, c.fin_ml};
-    for (void* p : ptrs) if (p) cudaFree(p);
+    if (c.block) cudaFree(c.block);
     if (c.pages) kata_pages_destroy(c.pages);
     delete h;
     return KATA_OK;

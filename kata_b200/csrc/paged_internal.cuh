@@ -19,11 +19,12 @@ struct PagedCtx {
     int page_shift = 4, width = 0;        // width: table entries per sequence
     int64_t rows_per_layer = 0;           // n_pages * page_size
     void* plane[KATA_PAGED_PLANES] = {}; bool owned[KATA_PAGED_PLANES] = {};
+    void* block = nullptr;                // one allocation for the pointers from d_table to scores
     int32_t* d_table = nullptr;           // [n_seqs][width], the device's copy of the page table
     RotTab* d_rot = nullptr;
     float* part_o = nullptr; float* part_ml = nullptr; int32_t* counters = nullptr; int32_t* d_err = nullptr;   // decode: partial rows of cut segments, their (m, l), tickets
     float* fin_ml = nullptr;              // decode with weights: joined (m, l) of every row of every segment
-    float* scores = nullptr;   // decode with weights: fp32 scores [tile][key][8 or 16 rows] of one launch
+    float* scores = nullptr;              // decode with weights: fp32 scores [tile][key][8 or 16 rows] of one launch
     std::vector<int32_t> stamp; int32_t stamp_now = 0;   // per sequence: the call it was last named in (finds a sequence named twice)
     CUtensorMap tm_k{}, tm_v{}; int box_groups = 1;     // rank-5 tile views of the K and V pools; 16-row groups per box
     int sm_count = 148;

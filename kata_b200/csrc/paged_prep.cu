@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(256, 3) paged_prep_kernel(const __grid_constan
     load_rows(h0);
     const int slot = b.slot[bi] + t; const int64_t row = paged_row(a.tables + (int64_t)b.seq[bi] * a.width, slot, a.page_shift);
     if (tid < a.rot_half) {
-        const int pos = a.axis_pos ? __ldg(a.axis_pos + tok * 3 + axis) : b.age[bi] + t;
+        const int pos = a.axis_pos ? __ldcg(a.axis_pos + tok * 3 + axis) : b.age[bi] + t;
         const float turn = (float)(int32_t)((freq * (uint64_t)(int64_t)pos) >> 32) * 0x1p-31f;   // in half circles, [-1, 1)
         sincospif(turn, &s_sin[tid], &s_cos[tid]);
     }
