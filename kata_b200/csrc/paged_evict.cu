@@ -189,6 +189,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_cluster_kernel(const
     pdl_wait(); pdl_launch_dependents();
     int32_t* src = a.src + (((int64_t)l * a.n + bi) * a.kv_heads + kvh) * keep;
     if (S <= keep) { for (int j = rank * kSelThreads + tid; j < keep; j += CS * kSelThreads) src[j] = j < S ? j : -1; return; }   // (the whole cluster)
+    cg::this_cluster().barrier_arrive();   // waited for before the first access to another CTA's shared memory: it has to have started
     const int32_t* table = a.tables + (int64_t)b.seq[bi] * a.width; const float* weight = a.weight + (int64_t)(a.layer0 + l) * a.plane_stride; const int32_t* age = a.age + (int64_t)(a.layer0 + l) * a.plane_stride;
     const int j0 = rank * wpc * 32, mine = min(max(S - j0, 0), wpc * 32), words = (mine + 31) >> 5;   // slots j0 .. j0 + mine - 1 are this CTA's; item i of a thread: j0 + tid + 512 * i
     constexpr bool REGS = ITEMS > 0;
@@ -232,6 +233,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_cluster_kernel(const
             hi = s_bound[0]; lo = min(s_bound[1], hi);
         };
         constexpr int step = kSelThreads * CS / kSample;
+        cg::this_cluster().barrier_wait();
         if (tid % step == 0) {   // every CTA's share of the sample, to every CTA
             uint32_t k = 0;
 #pragma unroll
@@ -298,6 +300,7 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_cluster_kernel(const
             if (found) { prefix = (uint32_t)s_bin; left = s_left; }
         }
     }
+    if (!REGS) cg::this_cluster().barrier_wait();
     if (!found) {   // ---- or by a radix select: digits of 8 bits, four histograms of 256 bins each, picked by lane (fewer lanes meet)
         for (int i = tid; i < 4 * 1024; i += kSelThreads) (&hist[0][0])[i] = 0;
         __syncthreads();
