@@ -8,8 +8,9 @@
 // clock per lane); then the words of 32 slots get their prefix sums by ballots and shuffles, the movers go to a list in shared memory in order, and every free slot
 // takes the mover of its rank.
 // select_cluster, above that: eight CTAs with a contiguous eighth of the slots each (one SM needs 12 us for the loads of 32K slots alone). Up to 131,072 slots the keys are in registers, and the
-// threshold is found by bounds: a sample of 512 keys gives two values that it hardly lies outside of (three standard deviations), the keys between them are gathered through distributed
-// shared memory, narrowed by a second sample and searched by one warp. Where the counts do not confirm the bounds, or too many keys lie between (one value shared
+// threshold is found by bounds: a sample of 512 keys gives two values that it hardly lies outside of (three standard deviations), the keys between them go to every CTA through distributed
+// shared memory, and each narrows them by counting at interpolated values until a warp can rank the rest (8 x 32K slots to 4,096 with the moves 70 us; narrowed by a second sample and
+// searched bit by bit by one warp 75). Where the counts do not confirm the bounds, or too many keys lie between (one value shared
 // by many slots), and for longer sequences, whose keys are read again in every pass, a radix select over the cluster's summed histograms finds it. Ranks of free slots and movers come
 // from prefix sums per word; the free slots are listed by rank where they lie, and each mover looks its own up.
 // move: a warp per 32 destinations, lanes agreeing by ballot on those that receive a row; each row is 16-byte copies of K and V. Bound by HBM: 2 x row bytes per move.
@@ -27,7 +28,7 @@ constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32;
 constexpr int kSelOne = 10 * kSelThreads, kSelMany = 64;   // one CTA per (layer, sequence, KV head) up to so many slots, or (up to 32,768) when there are so many of them: 256 times 8,000 slots took 36 us
                                                            // beside the move so, 180 us as clusters, whose latency then adds up
 constexpr int kSelCluster = 8, kCluSlots = kSelCluster * kSelThreads, kCluMax = 8 * kCluSlots;   // slots of a cluster per register of its threads; slots that it, or one CTA, selects from by bounds
-constexpr int kSample = kSelThreads, kOwn = 1024, kNear = 1024, kGather = 12;   // keys in a sample; keys that may lie between the bounds per CTA, after the second narrowing, and per thread of the gathered ones
+constexpr int kSample = kSelThreads, kOwn = 2 * kSelThreads;   // keys in the sample; keys that may lie between the bounds per CTA
 
 struct EvictArgs {
     int keep, sink, recent, width, page_shift, kv_heads, n, layer0;
@@ -181,11 +182,13 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_cluster_kernel(const
     namespace cg = cooperative_groups; constexpr int CS = kSelCluster;
     extern __shared__ __align__(16) uint32_t dyn[];
     uint32_t* kept = dyn; int32_t* pre_h = reinterpret_cast<int32_t*>(dyn + wpc); int32_t* pre_m = pre_h + wpc; uint16_t* list = reinterpret_cast<uint16_t*>(dyn + 3 * wpc);
-    __shared__ __align__(16) int32_t hist[4][1024]; __shared__ uint32_t own[kOwn], near[kNear], sample[kSample], s_bound[2]; __shared__ int32_t s_cand[CS], s_above[CS], s_eq[CS], s_holes[CS], s_movers[CS], s_sum[3], s_warp[kSelWarps]; __shared__ int s_bin, s_left, s_n[2];
+    // the keys between the bounds, of every CTA of the cluster; or the four histograms of the radix select
+    __shared__ __align__(16) uint32_t pool[ITEMS ? CS * kOwn : 4 * 1024]; int32_t* const hist = reinterpret_cast<int32_t*>(pool);
+    __shared__ uint32_t sample[kSample], s_bound[2]; __shared__ int32_t s_cand[CS], s_above[CS], s_eq[CS], s_holes[CS], s_movers[CS], s_sum[3], s_warp[kSelWarps]; __shared__ int s_bin, s_left, s_n;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rank = blockIdx.x % CS, kvh = blockIdx.x / CS, bi = blockIdx.y, l = blockIdx.z, S = b.slot[bi], keep = a.keep, newest = b.age[bi] - a.recent;   // ages from `newest` on are protected
     auto peer = [&](auto* p, int r) { return cg::this_cluster().map_shared_rank(p, r); };
     auto sync_all = [&]() { cg::this_cluster().sync(); };
-    if (tid == 0) { s_n[0] = s_n[1] = 0; s_sum[0] = s_sum[1] = s_sum[2] = 0; }
+    if (tid == 0) { s_n = s_left = 0; s_sum[0] = s_sum[1] = s_sum[2] = 0; }
     pdl_wait(); pdl_launch_dependents();
     int32_t* src = a.src + (((int64_t)l * a.n + bi) * a.kv_heads + kvh) * keep;
     if (S <= keep) { for (int j = rank * kSelThreads + tid; j < keep; j += CS * kSelThreads) src[j] = j < S ? j : -1; return; }   // (the whole cluster)
@@ -211,27 +214,14 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_cluster_kernel(const
         if (tid == 0) s_sum[turn == 2 ? 0 : turn + 1] = 0;   // read by everybody before this barrier, used after the next
         return t;
     };
-    auto slot_for = [&](int n, int which) {   // where a thread's n values go in a list counted by s_n[which]
+    auto slot_for = [&](int n) {   // where a thread's n values go in a list counted by s_n
         const int inc = warp_inclusive(n); int at = 0;
-        if (lane == 31 && inc) at = atomicAdd(&s_n[which], inc);
+        if (lane == 31 && inc) at = atomicAdd(&s_n, inc);
         return __shfl_sync(0xffffffffu, at, 31) + inc - n;
     };
     uint32_t prefix = 0; int left = keep;   // left: how many of the keys equal to prefix (of the keys that match it, on the way) are kept
     bool found = false;
     if constexpr (REGS) {   // ---- the keep-th largest key by bounds
-        auto bounds = [&](int target, int n, uint32_t& hi, uint32_t& lo) {   // where the target-th largest of n keys hardly lies above (hi) or below (lo), from the sample
-            if (w < 2) {   // warp 0 finds hi, warp 1 lo
-                uint32_t k[kSample / 32]; int n_s = 0;
-#pragma unroll
-                for (int i = 0; i < kSample / 32; i++) { k[i] = sample[i * 32 + lane]; n_s += k[i] != 0u; }
-                n_s = __reduce_add_sync(0xffffffffu, n_s);
-                const float f = (float)target / (float)n, mid = f * n_s, dev = 3.0f * sqrtf(n_s * f * (1.0f - f)) + 3.0f; const int t = w == 0 ? (int)(mid - dev) : (int)(mid + dev) + 1;   // rank in the sample
-                const uint32_t v = t < 1 ? 0xffffffffu : t > n_s ? 1u : warp_search(k, t, 1u, 0xffffffffu);
-                if (lane == 0) s_bound[w] = max(v, 1u);
-            }
-            __syncthreads();
-            hi = s_bound[0]; lo = min(s_bound[1], hi);
-        };
         constexpr int step = kSelThreads * CS / kSample;
         cg::this_cluster().barrier_wait();
         if (tid % step == 0) {   // every CTA's share of the sample, to every CTA
@@ -241,73 +231,77 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_cluster_kernel(const
             for (int r = 0; r < CS; r++) peer(&sample[0], r)[rank * (kSample / CS) + tid / step] = k;
         }
         sync_all();
-        uint32_t hi, lo; int up = 0, c = 0;
-        bounds(keep, S, hi, lo);
+        if (w < 2) {   // where the keep-th largest of the S keys hardly lies above (warp 0) or below (warp 1)
+            uint32_t k[kSample / 32]; int n_s = 0;
+#pragma unroll
+            for (int i = 0; i < kSample / 32; i++) { k[i] = sample[i * 32 + lane]; n_s += k[i] != 0u; }
+            n_s = __reduce_add_sync(0xffffffffu, n_s);
+            const float f = (float)keep / (float)S, mid = f * n_s, dev = 3.0f * sqrtf(n_s * f * (1.0f - f)) + 3.0f; const int t = w == 0 ? (int)(mid - dev) : (int)(mid + dev) + 1;   // rank in the sample
+            const uint32_t v = t < 1 ? 0xffffffffu : t > n_s ? 1u : warp_search(k, t, 1u, 0xffffffffu);
+            if (lane == 0) s_bound[w] = max(v, 1u);
+        }
+        __syncthreads();
+        const uint32_t hi = s_bound[0], lo = min(s_bound[1], hi); int up = 0, c = 0;
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) { up += key[i] > hi; c += key[i] >= lo && key[i] <= hi; }
-        int at = slot_for(c, 0);
+        int at = slot_for(c);
 #pragma unroll
-        for (int i = 0; i < ITEMS; i++) if (key[i] >= lo && key[i] <= hi) { if (at < kOwn) own[at] = key[i]; at++; }
+        for (int i = 0; i < ITEMS; i++) if (key[i] >= lo && key[i] <= hi) { if (at < kOwn) pool[rank * kOwn + at] = key[i]; at++; }
         up = total(up);
-        if (tid < CS) { peer(&s_cand[0], tid)[rank] = s_n[0]; peer(&s_above[0], tid)[rank] = up; }
+        for (int q = tid; q < min(s_n, kOwn); q += kSelThreads) {   // to the other CTAs
+            const uint32_t k = pool[rank * kOwn + q];
+            for (int r = 1; r < CS; r++) peer(&pool[0], (rank + r) % CS)[rank * kOwn + q] = k;
+        }
+        if (tid < CS) { peer(&s_cand[0], tid)[rank] = s_n; peer(&s_above[0], tid)[rank] = up; }
         sync_all();
         int above = 0, between = 0, most = 0;
 #pragma unroll
         for (int r = 0; r < CS; r++) { above += s_above[r]; between += s_cand[r]; most = max(most, s_cand[r]); }
-        int need = keep - above;   // the need-th largest of the keys between
-        found = most <= kOwn && between <= kGather * kSelThreads && need > 0 && need <= between;   // the same in every CTA of the cluster, as all that follows from it
-        if (found) {
-            auto cand = [&](int i) {   // key i of those between, whichever CTA found it
-                int r = 0;
-                while (r < CS - 1 && i >= s_cand[r]) i -= s_cand[r++];
-                return peer(&own[0], r)[i];
-            };
-            uint32_t k[kGather];
+        const int need = keep - above;   // the need-th largest of the keys between
+        found = most <= kOwn && need > 0 && need <= between;   // the same in every CTA of the cluster, as all that follows from it
+        if (found) {   // in every CTA by itself: n_from >= need of them reach `from`, n_to < need reach `to`; values between are tried, a little to either side of where the counts say that the key should lie (every
+            // fourth time halfway), until at most 32 keys are left for a warp to rank, or `from` is the key itself
+            constexpr int N = CS * kOwn / kSelThreads;
+            uint32_t k[N];
 #pragma unroll
-            for (int i = 0; i < kGather; i++) k[i] = tid + i * kSelThreads < between ? cand(tid + i * kSelThreads) : 0u;
-            if (between > kNear) {   // once more
-                sample[tid] = cand((int)((int64_t)tid * between / kSample));
+            for (int i = 0; i < N; i++) {
+                int q = tid + i * kSelThreads, r = 0; k[i] = 0u;
+                if (q < between) { while (q >= s_cand[r]) q -= s_cand[r++]; k[i] = pool[r * kOwn + q]; }
+            }
+            uint32_t from = lo, to = min(hi, 0xFF800000u) + 1u; int n_from = between, n_to = 0;   // (0xFF800000: the largest key)
+#pragma unroll 1
+            for (int step = 0; n_from - n_to > 32 && to - from > 1u; step++) {
+                const uint32_t gap = to - from; const int past = n_from - need > need - n_to ? n_from - need - 8 : n_from - need + 8;   // keys to leave behind
+                const uint32_t at = from + (step % 4 == 3 ? gap / 2 : min(max((uint32_t)((float)gap * ((float)past / (float)(n_from - n_to))), 1u), gap - 1u));
+                int c[4] = {};
+#pragma unroll
+                for (int i = 0; i < N; i++) if (i * kSelThreads < between) add_if_ge(c[i & 3], k[i], at);
+                const int n = total(c[0] + c[1] + c[2] + c[3]);
+                if (n >= need) { from = at; n_from = n; } else { to = at; n_to = n; }
+            }
+            prefix = from; left = need - n_to;   // `from` is one of many equal keys, unless
+            if (to - from > 1u) {
+#pragma unroll
+                for (int i = 0; i < N; i++) if (k[i] >= from && k[i] < to) sample[atomicAdd(&s_left, 1)] = k[i];
                 __syncthreads();
-                bounds(need, between, hi, lo);
+                const uint32_t mine_k = lane < n_from - n_to ? sample[lane] : 0u; int above_k = 0;   // every warp ranks them for itself
+#pragma unroll
+                for (int x = 0; x < 32; x++) above_k += __shfl_sync(0xffffffffu, mine_k, x) > mine_k;
+                // the largest key with fewer than `left` above it lies at rank `left`, ties included: the smallest of those
+                const uint32_t best = __reduce_min_sync(0xffffffffu, mine_k && above_k < left ? mine_k : 0xffffffffu);
+                const int over = __popc(__ballot_sync(0xffffffffu, mine_k > best));
+                prefix = best; left -= over;
             }
-            int u = 0, n = 0;
-#pragma unroll
-            for (int i = 0; i < kGather; i++) { u += k[i] > hi; n += k[i] >= lo && k[i] <= hi; }
-            int to = slot_for(n, 1);
-#pragma unroll
-            for (int i = 0; i < kGather; i++) if (k[i] >= lo && k[i] <= hi) { if (to < kNear) near[to] = k[i]; to++; }
-            u = total(u);
-            const int m = s_n[1];
-            need -= u; found = m <= kNear && need > 0 && need <= m;
-            if (found && w == 0) {
-                auto last = [&](auto size) {   // over 32 * N keys
-                    constexpr int N = decltype(size)::value;
-                    uint32_t x[N], least = 0xffffffffu; int g = 0;
-#pragma unroll
-                    for (int i = 0; i < N; i++) x[i] = i * 32 + lane < m ? near[i * 32 + lane] : 0u;
-                    const uint32_t v = warp_search(x, need, lo, hi);
-#pragma unroll
-                    for (int i = 0; i < N; i++) if (x[i] >= v && x[i] != 0u) least = min(least, x[i]);   // the smallest key that reaches it: the threshold
-                    least = __reduce_min_sync(0xffffffffu, least);
-#pragma unroll
-                    for (int i = 0; i < N; i++) g += x[i] > least;
-                    g = __reduce_add_sync(0xffffffffu, g);
-                    if (lane == 0) { s_bin = (int)least; s_left = need - g; }
-                };
-                if (m <= 256) last(std::integral_constant<int, 8>()); else if (m <= 512) last(std::integral_constant<int, 16>()); else last(std::integral_constant<int, kNear / 32>());
-            }
-            __syncthreads();
-            if (found) { prefix = (uint32_t)s_bin; left = s_left; }
         }
     }
     if (!REGS) cg::this_cluster().barrier_wait();
     if (!found) {   // ---- or by a radix select: digits of 8 bits, four histograms of 256 bins each, picked by lane (fewer lanes meet)
-        for (int i = tid; i < 4 * 1024; i += kSelThreads) (&hist[0][0])[i] = 0;
+        for (int i = tid; i < 4 * 1024; i += kSelThreads) hist[i] = 0;
         __syncthreads();
         uint32_t mask = 0;
 #pragma unroll 1
         for (int pass = 0; pass < 4; pass++) {
-            const int shift = 24 - 8 * pass; int32_t* hp = hist[pass];
+            const int shift = 24 - 8 * pass; int32_t* hp = hist + pass * 1024;
             each([&](uint32_t k, int) { if (k != 0u && (k & mask) == prefix) atomicAdd(&hp[((k >> shift) & 255u) * 4 + (lane & 3)], 1); });
             sync_all();
             int c = 0;   // thread t < 256: bin 255 - t
@@ -356,12 +350,20 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_cluster_kernel(const
     // ---- movers: the free slot of the same rank, wherever in the cluster it lies
     int rk0 = 0;
     for (int r = 0; r < rank; r++) rk0 += s_movers[r];
-    for (int q = max(keep - j0, 0) + tid; q < mine; q += kSelThreads) {
-        const int wd = q >> 5; const uint32_t bit = 1u << (q & 31);
-        if (!(kept[wd] & bit)) continue;
-        int rk = rk0 + pre_m[wd] + __popc(kept[wd] & ~below(wd) & (bit - 1)), r = 0;
-        while (r < CS - 1 && rk >= s_holes[r]) rk -= s_holes[r++];
-        src[r * wpc * 32 + peer(list, r)[rk]] = j0 + q;
+    for (int q0 = max(keep - j0, 0) + tid; q0 < mine; q0 += 4 * kSelThreads) {   // four at a time: the reads of other CTAs' lists are under way together
+        int at[4]; uint32_t to[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int q = q0 + u * kSelThreads, wd = q >> 5; const uint32_t bit = 1u << (q & 31);
+            at[u] = -1;
+            if (q < mine && (kept[wd] & bit)) {
+                int rk = rk0 + pre_m[wd] + __popc(kept[wd] & ~below(wd) & (bit - 1)), r = 0;
+                while (r < CS - 1 && rk >= s_holes[r]) rk -= s_holes[r++];
+                at[u] = r * wpc * 32; to[u] = peer(list, r)[rk];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) if (at[u] >= 0) src[at[u] + to[u]] = j0 + q0 + u * kSelThreads;
     }
     sync_all();   // nobody leaves while its shared memory may still be read
 }
@@ -404,7 +406,8 @@ __global__ void __launch_bounds__(256) paged_move_kernel(const __grid_constant__
 }  // namespace
 
 cudaError_t configure_paged_evict(const PagedCtx&) {   // shared-memory opt-in, per device
-    const cudaError_t e = cudaFuncSetAttribute(paged_select_cluster_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, KATA_PAGED_MAX_SLOTS / 32 / kSelCluster * 76);
+    cudaError_t e = cudaFuncSetAttribute(paged_select_cluster_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCluMax / 32 / kSelCluster * 76);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(paged_select_cluster_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, KATA_PAGED_MAX_SLOTS / 32 / kSelCluster * 76);
     return e != cudaSuccess ? e : cudaFuncSetAttribute(paged_select_cluster_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kCluMax / 32 / kSelCluster * 76);
 }
 
