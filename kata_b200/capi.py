@@ -475,6 +475,7 @@ class PagedContext:
         ("k", "v", "k_scale", "v_scale", "weight", "age") in the header's layout, [n_layers] of them; the others are allocated, zero-filled."""
         L = self.L = lib()
         self.device = torch.cuda.current_device() if device is None else device
+        self.cuda = torch.device("cuda", self.device)
         self.n_layers, self.n_seqs, self.n_pages, self.page_size, self.max_slots = n_layers, n_seqs, n_pages, page_size, max_slots
         self.heads, self.kv_heads, self.head_dim, self.kv_mode, self.gated, self.weights = heads, kv_heads, head_dim, kv_mode, gated, weights
         if kv_mode not in _KV_MODES:
@@ -555,7 +556,7 @@ class PagedContext:
 
         class _Alias:
             __cuda_array_interface__ = {"shape": shape, "typestr": kind, "data": (ptr, False), "version": 3, "strides": None}
-        return torch.as_tensor(_Alias(), device=torch.device("cuda", self.device))
+        return torch.as_tensor(_Alias(), device=self.cuda)
 
     # ---- the operators
     def _at(self, what, t, n, kinds):
@@ -576,8 +577,8 @@ class PagedContext:
         qp = gp = hp = None
         if q is not None:
             qp = self._at("q", q, nq * (2 if self.gated else 1), act)
-            q16 = torch.empty((n, T, self.heads * D), dtype=torch.float16, device=k.device) if q16 is None else q16
-            gate = torch.empty((n, T, self.heads * D), dtype=torch.float32, device=k.device) if gate is None and self.gated else gate
+            q16 = torch.empty(n, T, self.heads * D, dtype=torch.float16, device=k.device) if q16 is None else q16   # (sizes one by one: a microsecond less than as a tuple)
+            gate = torch.empty(n, T, self.heads * D, dtype=torch.float32, device=k.device) if gate is None and self.gated else gate
             hp = self._at("q16", q16, nq, _F16)
         if gate is not None:
             gp = self._at("gate", gate, nq, _F32)
@@ -595,7 +596,7 @@ class PagedContext:
             raise ValueError("one n_slots per sequence")
         nq = n * T * self.heads * self.head_dim
         qp = self._at("q16", q16, nq, _F16)
-        out = torch.empty((n, T, self.heads * self.head_dim), dtype=out_dtype, device=q16.device) if out is None else out
+        out = torch.empty(n, T, self.heads * self.head_dim, dtype=out_dtype, device=q16.device) if out is None else out
         rc = self.L.kata_paged_decode(self.h, layer, n, ids.buffer_info()[0], held.buffer_info()[0], T, qp, None if gate is None else self._at("gate", gate, nq, _F32), self._at("out", out, nq, _ACT), _ACT[out.dtype], 1 if accumulate else 0, self._s())
         if rc:
             self._ck(rc)
@@ -610,7 +611,7 @@ class PagedContext:
         if len(held) != n or len(total) != n:
             raise ValueError("one n_slots (and seen) per sequence")
         shape = (n, self.kv_heads, keep) if n_layers == 1 else (n_layers, n, self.kv_heads, keep)
-        src = torch.empty(shape, dtype=torch.int32, device=torch.device("cuda", self.device)) if src is None else src
+        src = torch.empty(*shape, dtype=torch.int32, device=self.cuda) if src is None else src
         rc = self.L.kata_paged_evict(self.h, layer, n_layers, n, ids.buffer_info()[0], held.buffer_info()[0], total.buffer_info()[0], keep, sink, recent, self._at("src", src, n_layers * n * self.kv_heads * keep, _I32), self._s())
         if rc:
             self._ck(rc)
