@@ -16,7 +16,7 @@
 //    of its own, whose lanes fetch the slots' K and V scales as well, three tiles ahead, and leave them in shared memory: the score warp waited when it had the loads (359 us for 32 sequences of 300 to
 //    32K slots, 228 with a producer per ring, all else as it was then), and so it did with one warp for the four rings' scales (352 us).
 //  - Groups behind the last slot repeat the last page (their table entry may not exist); such slots are masked, and their V rows zeroed in shared
-//    memory, so whatever lies there (NaN included) has no part in the result.
+//    memory, so whatever lies there (NaN included) has no part in the result. Nor has the row of a later token in an earlier one's.
 // Head layouts: head_dim 256 or 128, up to 16 query heads per KV head; tokens beyond 16 / group run as further passes.
 //
 // The matrix instructions take the keys (and the head dims of V) as their 16 rows and the query rows as their 8 columns: S^T = K Q^T, O^T = V^T P^T. One token of up to 8 heads
@@ -53,9 +53,10 @@ template <int HD, bool K8, int NR> struct PGeo {   // NR: column tiles of 8 quer
     static constexpr int kPStride = 32 * kNK + 16, kPTerm = NR * 8 * kPStride, kPBytes = 2 * kPTerm + 64;   // a P slot: two fp16 blocks (heads and remainders), 16 rescale factors
     static constexpr int kPShift = K8 ? 5 : 15;                                          // p is carried as 2^kPShift * p (int8: p times a scale up to 516 has to stay below 65504)
     static constexpr int kAcc = HD / 32 * NR * 4, kRedBytes = 2 * kAcc * 128;            // accumulators per value-warp lane; the block in which the rings add them up
+    // (m, l) of every ring's rows, of their join, and (int8) what a ring's rows of O are multiplied by when they are joined.
     // NR = 1: a block of its own, and two slots for the rings' (m, l): the score warps go on into the next segment. NR = 2: no room, it lies where the P slots are and the score warps wait.
     static constexpr int kSums = NR == 1 ? 2 : 1;
-    static constexpr int kOffBars = kQBytes, kOffMl = kOffBars + kBarBytes, kOffPair = kOffMl + kSums * 512 + 128, kOffRed = kOffPair + (NR == 1 ? kRings * 2 * kPBytes : 0);
+    static constexpr int kOffBars = kQBytes, kOffMl = kOffBars + kBarBytes, kOffPair = kOffMl + kSums * (512 + (K8 ? 256 : 0)) + 128, kOffRed = kOffPair + (NR == 1 ? kRings * 2 * kPBytes : 0);
     static constexpr int kOffScale = NR == 1 ? kOffRed + kRedBytes : kOffPair + (kRings * 2 * kPBytes > kRedBytes ? kRings * 2 * kPBytes : kRedBytes), kOffStages = kOffScale + (K8 ? kRings * kStages * kTile * 4 : 0);   // scales: [ring][stage][slot] K and V packed
     static constexpr int kSmem = kOffStages + 1024 + kRings * kRingBytes;
     static_assert(kSmem <= 232448, "shared memory");
@@ -271,6 +272,45 @@ __device__ __forceinline__ void paged_values(const uint32_t v_sm, const uint32_t
     }
 }
 
+// Value warp, the last tiles of an fp16 segment, half vh of the head dims: slots [0, part) are seen by every token of the pass, [part, nk) by some, the others by none. The rows that no token sees become zeros
+// (0 x NaN is not 0; int8 codes are finite whatever they are). In those that some see, infinities and NaN become zeros, and what comes of them (the two terms of P make NaN of either) goes into the
+// rows of O that see them: bit 16 * y + x of the result says that dim 8 * x + g of column 8 * (y >> 1) + 2 * t4 + (y & 1) is NaN. all_see: as in the kernel, less the tile's first slot. The caller
+// puts them in once it is through with its tiles: in the loop the registers are missing (one sequence of 32K slots 30.9 us instead of 29.6).
+template <int HD, int NR>
+__device__ __forceinline__ uint64_t clean_v_rows(uint8_t* v, int part, int nk, int all_see, int group, int lane, int vh) {
+    using G = PGeo<HD, false, NR>; constexpr int kHC = HD / 16;   // 16-byte chunks of half a head row
+    auto chunk = [&](int r, int c) { c += vh * kHC; return v + (r >> 4) * G::kGroupBytes + (c >> 3) * 2048 + (r & 15) * 128 + (((c & 7) ^ (r & 7)) << 4); };
+    auto odd = [](uint32_t h) { return (h & 0x7c00u) == 0x7c00u; };
+#pragma unroll 1
+    for (int i = lane; i < (G::kTile - nk) * kHC; i += 32) *reinterpret_cast<uint4*>(chunk(nk + i / kHC, i % kHC)) = make_uint4(0, 0, 0, 0);
+    bool any = false;
+    uint64_t bad = 0;
+#pragma unroll 1
+    for (int i = lane; i < (nk - part) * kHC; i += 32) {
+        const uint4 x = *reinterpret_cast<const uint4*>(chunk(part + i / kHC, i % kHC));
+        any = any || odd(x.x) || odd(x.x >> 16) || odd(x.y) || odd(x.y >> 16) || odd(x.z) || odd(x.z >> 16) || odd(x.w) || odd(x.w >> 16);
+    }
+    if (__any_sync(0xffffffffu, any)) {
+#pragma unroll 1
+        for (int r = part; r < nk; r++) {
+            uint64_t dims = 0;
+#pragma unroll 1
+            for (int x = 0; x < kHC; x++) dims |= (uint64_t)odd(*reinterpret_cast<const unsigned short*>(chunk(r, x) + 2 * (lane >> 2))) << x;
+#pragma unroll 1
+            for (int y = 0; y < 2 * NR; y++) if (r < all_see + ((y >> 1) * 8 + 2 * (lane & 3) + (y & 1)) / group) bad |= dims << (16 * y);   // token t sees slots below all_see + t
+        }
+        __syncwarp();
+#pragma unroll 1
+        for (int i = lane; i < (nk - part) * kHC * 8; i += 32) {
+            unsigned short* h = reinterpret_cast<unsigned short*>(chunk(part + i / (kHC * 8), i / 8 % kHC)) + i % 8;
+            if (odd(*h)) *h = 0;
+        }
+    }
+    fence_proxy_async();   // generic writes to a stage that TMA fills again
+    __syncwarp();
+    return bad;
+}
+
 struct PagedOut { const float* gate; void* out; int32_t kind; float* fin_ml; };   // fin_ml: joined (m, 1 / l) per (segment, row), with weights only
 
 // Final value of row r of a segment, dims d and d + 1: normalised, gated, stored. A row that saw no slot has L = 0 and gets zeros.
@@ -421,7 +461,7 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
         const int kend = p.kend[b];
         const int n_mine = n_here > ring ? (n_here - ring + kRings - 1) / kRings : 0;   // this ring's tiles: lt0 + ring, lt0 + ring + 4, ...
         const uint32_t it_seg = it, sums = n_segs % G::kSums, sums_par = (n_segs / G::kSums) & 1u;
-        float* ml_seg = sm_ml + sums * kRings * 32;
+        float* ml_seg = sm_ml + sums * kRings * 32; float* factor = joined_ml + 32 + sums * kRings * 16;
         const int all_see = kend - p.T + 1;   // slots below this are seen by every row (columns that hold no query too: nobody reads what they get)
 
         if (h == 0) {
@@ -437,7 +477,7 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
             for (int x = 0; x < kQLoads; x++) { const int ch = tid + x * 128; stage_q_chunk<K8>(smem + ch / (HD / 8) * G::kQStride, ch % (HD / 8), qv[x]); }
             score_sync();
             if (!dead && !mbar_wait_bounded(sempty + sums * 8, sums_par ^ 1u, err)) { dead = true; atomicExch(err, 6); }   // the sums of kSums segments ago have been read
-            RowsState<NR> ss; int lim[NR][2]; uint32_t qf[HD / 16][2];
+            RowsState<NR> ss; int lim[NR][2]; uint32_t qf[HD / 16][2], spoilt = 0;
 #pragma unroll
             for (int nr = 0; nr < NR; nr++)
 #pragma unroll
@@ -464,6 +504,18 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ebars + stg * 8);   // K and the scales (in registers by now) of this stage are no longer needed
                 if (key0 + kTile > all_see) {   // masked by select: what lies behind the last slot may be anything
+                    if (K8) {   // a V scale of infinity or NaN: 0 x that is not 0. The rows that see it become NaN when the rings are joined
+#pragma unroll
+                        for (int sb = 0; sb < NK; sb++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                const int slot_no = key0 + 16 * sb + 8 * e + g;
+                                if (slot_no < all_see || (sc[sb][e] & 0x7c000000u) != 0x7c000000u) continue;
+                                sc[sb][e] &= 0xffffu;
+#pragma unroll
+                                for (int x = 0; x < 2 * NR; x++) if (slot_no < lim[x >> 1][x & 1]) spoilt |= 1u << x;
+                            }
+                    }
 #pragma unroll
                     for (int sb = 0; sb < NK; sb++)
 #pragma unroll
@@ -503,26 +555,23 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
                     float l = ss.l[nr][e];
                     l += __shfl_xor_sync(0xffffffffu, l, 4); l += __shfl_xor_sync(0xffffffffu, l, 8); l += __shfl_xor_sync(0xffffffffu, l, 16);
                     if (g == 0) *reinterpret_cast<float2*>(ml_seg + (ring * 16 + nr * 8 + 2 * t4 + e) * 2) = make_float2(ss.m[nr][e], l);
+                    if (K8 && g == 0) factor[ring * 16 + nr * 8 + 2 * t4 + e] = 1.0f;
                 }
+            __syncwarp();
+            if (K8 && spoilt) {
+#pragma unroll 1
+                for (int x = 0; x < 2 * NR; x++) if (spoilt >> x & 1u) factor[ring * 16 + (x >> 1) * 8 + 2 * t4 + (x & 1)] = NAN;
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(sfull + sums * 8);
         } else {
-            const int vh = h - 1; ValueAcc<HD, NR> vst; vst.clear();
+            const int vh = h - 1; ValueAcc<HD, NR> vst; vst.clear(); uint64_t bad = 0;
             for (int i = 0; i < n_mine; i++) {
                 const uint32_t cur = it_seg + (uint32_t)i, stg = cur % kStages, par = (cur / kStages) & 1u, slot = cur & 1u;
                 const uint32_t vt = ring_stage0 + stg * G::kStageBytes + G::kHalfBytes;
                 const int key0 = (lt0 + ring + i * kRings) * kTile;
                 if (!dead && !mbar_wait_bounded(bars + stg * 8, par, err)) { dead = true; atomicExch(err, 1); }
-                if (!K8 && key0 + kTile > kend) {   // the V rows behind the last slot become zeros (0 x NaN is not 0; int8 codes are finite whatever they are)
-                    const int nk = max(0, kend - key0);
-                    constexpr int kHC = G::kRowBytes / 32;   // 16-byte chunks of half a head row
-                    for (int idx = lane; idx < (kTile - nk) * kHC; idx += 32) {
-                        const int r = nk + idx / kHC, c = vh * kHC + idx % kHC;
-                        *reinterpret_cast<uint4*>(smem + (vt - sm_base) + (r >> 4) * G::kGroupBytes + (c >> 3) * 2048 + (r & 15) * 128 + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async();   // generic writes to a stage that TMA fills again
-                    __syncwarp();
-                }
+                if (!K8 && key0 + kTile > all_see) bad |= clean_v_rows<HD, NR>(smem + (vt - sm_base), max(0, all_see - key0), max(0, min(kend - key0, kTile)), all_see - key0, p.group, lane, vh);   // at most the ring's last tile
                 if (!dead && !mbar_wait_bounded(pfull + slot * 8, (cur >> 1) & 1u, err)) { dead = true; atomicExch(err, 5); }
                 const float* alpha = reinterpret_cast<const float*>(smem + p_off + (slot + 1) * G::kPBytes - 64);
                 if (!K8 || p.two_terms) paged_values<HD, K8, NR, true>(vt, sm_base + p_off + slot * G::kPBytes, alpha, vst, lane, vh); else paged_values<HD, K8, NR, false>(vt, sm_base + p_off + slot * G::kPBytes, alpha, vst, lane, vh);
@@ -531,6 +580,12 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
             }
             // ---- join the four rings: ring 3 leaves its rows of O^T, scaled to the joint maximum, where the P slots were, ring 2 adds its own, ring 1, ring 0. The same lane holds the same
             // dims and rows in every ring, and the order is fixed. The producers are in the next segment meanwhile.
+            if (!K8 && bad != 0) {
+#pragma unroll
+                for (int x = 0; x < HD / 16; x++)
+#pragma unroll
+                    for (int y = 0; y < 2 * NR; y++) if (bad >> (16 * y + x) & 1u) vst.o[x >> 1][y >> 1][2 * (x & 1) + (y & 1)] = NAN;
+            }
             if (!dead && !mbar_wait_bounded(sfull + sums * 8, sums_par, err)) { dead = true; atomicExch(err, 7); }   // the rings' (m, l) are there
             value_sync();   // the segment before has left the block (NR = 2: and P is read)
 #pragma unroll
@@ -546,6 +601,7 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
                         l += ml_seg[(ww * 16 + r) * 2 + 1] * wt;
                         if (ww == ring) mine = wt;
                     }
+                    if (K8 && mine != 0.0f) mine *= factor[ring * 16 + r];
                     if (ring == 0 && vh == 0 && g == 0) *reinterpret_cast<float2*>(joined_ml + r * 2) = make_float2(mx, l);
 #pragma unroll
                     for (int j = 0; j < HD / 32; j++) { vst.o[j][nr][e] = mine == 0.0f ? 0.0f : vst.o[j][nr][e] * mine; vst.o[j][nr][2 + e] = mine == 0.0f ? 0.0f : vst.o[j][nr][2 + e] * mine; }
