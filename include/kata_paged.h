@@ -101,7 +101,8 @@ int kata_paged_prep(kata_paged_ctx* ctx, int32_t layer, int32_t n, const int32_t
 
 /* Attention of the T newest tokens of each sequence (1..KATA_MAX_VERIFY) over its n_slots[b] slots: token t sees slots [0, n_slots[b] - T + 1 + t).
  *   d_out [n][T][heads][head_dim] out_dtype = softmax(q k^T) v (* sigmoid(gate) when d_gate is given); a token that sees no slot gets zeros.
- * The probabilities go into the matrix product in two fp16 terms (about 22 bits); for int8 caches with bf16 or fp16 outputs in one (2^-11 relative).
+ * The probabilities go into the matrix product in two fp16 terms (about 22 bits); for int8 caches with bf16 or fp16 outputs in one (2^-11 relative). They are carried relative to the
+ * row's largest probability so far and, int8, times the V scale relative to the largest of its tile of 32 or 64 slots, whatever the size of either; parts below 2^-40 of these are lost.
  * accumulate != 0 (KATA_PAGED_WEIGHTS; each sequence once per call): weight[head][slot] += the slot's probability, summed over the tokens and over the
  * query heads of the KV head. No atomics: the sums come out the same in every run. */
 int kata_paged_decode(kata_paged_ctx* ctx, int32_t layer, int32_t n, const int32_t* seq_ids, const int32_t* n_slots, int32_t T,

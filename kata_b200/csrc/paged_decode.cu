@@ -24,7 +24,9 @@
 // for the whole segment. With the query rows as the 16 rows instead, 32 sequences of 300 to 32K int8 slots took 280 us (228 at that time).
 //
 // Precision: fp16 products, fp32 sums. The exponent carries an offset (kPShift) so that p lies high in fp16's range: it cancels in p / l and keeps
-// small p out of the subnormals. p goes into P.V in two fp16 terms (about 22 bits; int8 caches with 16-bit outputs: one term, 2^-11 relative, there the second costs time), int8 codes are taken
+// small p out of the subnormals. p goes into P.V in two fp16 terms (about 22 bits; int8 caches with 16-bit outputs: one term, 2^-11 relative, there the second costs time), for int8 caches times the slot's V scale in units of
+// a power of two above the largest V scale of the tile: O and alpha carry the units from tile to tile, so small values keep as many bits as large ones (with the bare scale, whose products sank into fp16's subnormals, outputs
+// were off by 1e-5 at V scales of 1e-3 and by 1 % at 1e-6). What is lost lies below 2^-40 of the row's heaviest p times the tile's largest scale. int8 codes are taken
 // without the 1152 bias of the contiguous kernel (whose subtraction costs some ten bits), and a tile's P.V is formed in fresh accumulators and added to O with a rounded fma (the matrix
 // unit truncates its sums: over hundreds of tiles that showed as 3e-6 in fp32 outputs).
 #include <algorithm>
@@ -51,7 +53,7 @@ template <int HD, bool K8, int NR> struct PGeo {   // NR: column tiles of 8 quer
     static constexpr int kRingBytes = kStages * kStageBytes;
     static constexpr int kQStride = HD * 2 + 16, kQBytes = NR * 8 * kQStride;                // the query block: fp16 rows, 16 bytes of padding
     static constexpr int kPStride = 32 * kNK + 16, kPTerm = NR * 8 * kPStride, kPBytes = 2 * kPTerm + 64;   // a P slot: two fp16 blocks (heads and remainders), 16 rescale factors
-    static constexpr int kPShift = K8 ? 5 : 15;                                          // p is carried as 2^kPShift * p (int8: p times a scale up to 516 has to stay below 65504)
+    static constexpr int kPShift = 15;                                                   // p is carried as 2^kPShift * p (int8: times a scale below 1)
     static constexpr int kAcc = HD / 32 * NR * 4, kRedBytes = 2 * kAcc * 128;            // accumulators per value-warp lane; the block in which the rings add them up
     // (m, l) of every ring's rows, of their join, and (int8) what a ring's rows of O are multiplied by when they are joined.
     // NR = 1: a block of its own, and two slots for the rings' (m, l): the score warps go on into the next segment. NR = 2: no room, it lies where the P slots are and the score warps wait.
@@ -477,7 +479,7 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
             for (int x = 0; x < kQLoads; x++) { const int ch = tid + x * 128; stage_q_chunk<K8>(smem + ch / (HD / 8) * G::kQStride, ch % (HD / 8), qv[x]); }
             score_sync();
             if (!dead && !mbar_wait_bounded(sempty + sums * 8, sums_par ^ 1u, err)) { dead = true; atomicExch(err, 6); }   // the sums of kSums segments ago have been read
-            RowsState<NR> ss; int lim[NR][2]; uint32_t qf[HD / 16][2], spoilt = 0;
+            RowsState<NR> ss; int lim[NR][2], o_unit = 127; uint32_t qf[HD / 16][2], spoilt = 0;   // o_unit: O is carried in units of 2^(o_unit - 127) (int8)
 #pragma unroll
             for (int nr = 0; nr < NR; nr++)
 #pragma unroll
@@ -533,14 +535,23 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
                             for (int e = 0; e < 2; e++) *reinterpret_cast<float2*>(st + (16 * sb + 8 * e) * srow + nr * 8) = make_float2(s[sb][nr][2 * e], s[sb][nr][2 * e + 1]);
                 }
                 paged_softmax<NK, NR, G::kPShift>(s, ss, al);
-                if (K8) {
+                if (K8) {   // P holds p times the V scale in units of 2^(exponent of the tile's largest + 1), so that it fills fp16's range whatever the size of the values; O follows from tile to tile by alpha
+                    float vs[NK][2], top = 0.0f;
+#pragma unroll
+                    for (int sb = 0; sb < NK; sb++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) { vs[sb][e] = __half2float(__ushort_as_half((unsigned short)(sc[sb][e] >> 16))); top = fmaxf(top, fabsf(vs[sb][e])); }
+                    const int unit = min(max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23), 103), 143) + 1;   // biased; 2^-24 is the smallest scale, infinity counts as 2^16
+                    const float inv = __uint_as_float((uint32_t)(254 - unit) << 23), turn = __uint_as_float((uint32_t)(127 + o_unit - unit) << 23);
+                    o_unit = unit;
+#pragma unroll
+                    for (int nr = 0; nr < NR; nr++) { al[nr][0] *= turn; al[nr][1] *= turn; }
 #pragma unroll
                     for (int sb = 0; sb < NK; sb++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const float v = __half2float(__ushort_as_half((unsigned short)(sc[sb][e >> 1] >> 16)));
 #pragma unroll
-                            for (int nr = 0; nr < NR; nr++) s[sb][nr][e] *= v;
+                            for (int nr = 0; nr < NR; nr++) s[sb][nr][e] *= vs[sb][e >> 1] * inv;
                         }
                 }
                 if (cur >= 2 && !dead && !mbar_wait_bounded(pempty + slot * 8, ((cur >> 1) - 1u) & 1u, err)) { dead = true; atomicExch(err, 4); }
@@ -555,7 +566,7 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
                     float l = ss.l[nr][e];
                     l += __shfl_xor_sync(0xffffffffu, l, 4); l += __shfl_xor_sync(0xffffffffu, l, 8); l += __shfl_xor_sync(0xffffffffu, l, 16);
                     if (g == 0) *reinterpret_cast<float2*>(ml_seg + (ring * 16 + nr * 8 + 2 * t4 + e) * 2) = make_float2(ss.m[nr][e], l);
-                    if (K8 && g == 0) factor[ring * 16 + nr * 8 + 2 * t4 + e] = 1.0f;
+                    if (K8 && g == 0) factor[ring * 16 + nr * 8 + 2 * t4 + e] = __uint_as_float((uint32_t)o_unit << 23);
                 }
             __syncwarp();
             if (K8 && spoilt) {
