@@ -117,7 +117,8 @@ int kata_paged_evict(kata_paged_ctx* ctx, int32_t layer, int32_t n_layers, int32
                      int32_t* d_src, void* stream);
 
 /* Copies n_rows cache rows of a contiguous context (sequence src_seq, layer src_layer, positions src_pos ..) into slots slot0 .. of a sequence: a prompt
- * that kata_attn_prefill has worked on goes on in pages. Same kv_mode, 24 heads, 4 KV heads, head_dim 256, same device. Weights start at 0, ages at age0. */
+ * that kata_attn_prefill has worked on goes on in pages. Same kv_mode, 24 heads, 4 KV heads, head_dim 256, same device; KATA_ERR_MODE for a source
+ * that kata_attn_set_kv_heads has restricted (it never wrote the other heads' rows). Weights start at 0, ages at age0. */
 int kata_paged_import(kata_paged_ctx* ctx, int32_t layer, int32_t seq, int32_t slot0, int32_t n_rows, int32_t age0, kata_attn_ctx* src, int32_t src_layer, int32_t src_seq, int32_t src_pos, void* stream);
 
 /* How a decode launch would be shared out (host only, no GPU): tile_keys (16, 32 or 64) keys per tile, the tiles of all (sequence, KV head) segments in one list, CTA c works on tiles

@@ -249,6 +249,7 @@ int kata_paged_import(kata_paged_ctx* h, int32_t layer, int32_t seq, int32_t slo
     if (!src) return pfail(c, KATA_ERR_ARG, "import needs a source context");
     kata::Ctx& a = kata::ctx_of(src);
     if (c.cfg.heads != KATA_HEADS || c.cfg.kv_heads != KATA_KV_HEADS || c.cfg.head_dim != KATA_HEAD_DIM || a.cfg.kv_mode != c.cfg.kv_mode || a.cfg.device != c.cfg.device) return pfail(c, KATA_ERR_MODE, "import needs the same head layout, cache mode and device on both sides");
+    if (a.kvh_n != KATA_KV_HEADS) return pfail(c, KATA_ERR_MODE, "import takes rows of all %d KV heads (the source context writes %d of them)", KATA_KV_HEADS, a.kvh_n);
     if (n_rows < 1) return pfail(c, KATA_ERR_RANGE, "import of %d rows", n_rows);
     if (int rc = check_batch(c, layer, 1, 1, &seq, &slot0, true)) return rc;
     if (int rc = check_slots(c, seq, slot0, (int64_t)slot0 + n_rows)) return rc;

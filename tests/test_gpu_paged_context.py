@@ -1,0 +1,26 @@
+"""capi.PagedContext beside what surrounds it: contexts that rows are taken over from, tensors that alias its planes, ages after an eviction."""
+import pytest
+import torch
+
+from .test_gpu_paged import _context, _gen, _randn, capi  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def test_import_refuses_a_source_that_writes_some_of_the_kv_heads(capi):  # noqa: F811
+    g = _gen(21)
+    arena, ctx = capi.AttnContext(1, [64]), _context(capi, [40])
+    kn, k = 1 + 0.05 * _randn(g, 256), _randn(g, 1, 20, 1024)
+    ctx.plane(0, "k").fill_(3.0)
+    arena.prep(0, [0], [0], 20, None, k, k, None, kn, h0=24, nh=8)
+    for lo, n in ((0, 2), (3, 1)):
+        arena.set_kv_heads(lo, n)
+        with pytest.raises(capi.KataError) as e:
+            ctx.import_rows(0, 0, 0, 20, arena, 0, 0, 0)
+        assert e.value.code == 3
+        torch.cuda.synchronize()
+        assert (ctx.plane(0, "k") == 3).all()
+    arena.set_kv_heads(0, 4)
+    ctx.import_rows(0, 0, 0, 20, arena, 0, 0, 0)
+    assert not (ctx.plane(0, "k") == 3).all()
+    ctx.check()
