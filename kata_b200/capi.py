@@ -100,6 +100,28 @@ def out_fwht(x, sign, out=None):
     return out
 
 
+class _Native:
+    """A native context. It is destroyed when the last that holds it is gone: the Python object, by close(), or a tensor that aliases its memory."""
+
+    def __init__(self, destroy, h):
+        self.destroy, self.h = destroy, h
+
+    def __del__(self):
+        try:
+            self.destroy(self.h)
+        except Exception:
+            pass
+
+
+def _alias(native, ptr, shape, kind, device):
+    """A tensor over a native context's memory; torch keeps the interface object, and with it the context, as long as the storage lives."""
+    class _Memory:
+        __cuda_array_interface__ = {"shape": shape, "typestr": kind, "data": (ptr, False), "version": 3, "strides": None}
+    memory = _Memory()
+    memory.native = native
+    return torch.as_tensor(memory, device=device)
+
+
 class AttnContext:
     """One context per GPU: the KV caches of ``len(max_ctx)`` sequences x ``n_layers`` layers plus all scratch."""
 
@@ -116,11 +138,10 @@ class AttnContext:
         rc = self.L.kata_attn_create(C.byref(cfg), C.byref(self.h))
         if rc != OK:
             raise KataError(rc, "kata_attn_create failed")
+        self._native = _Native(self.L.kata_attn_destroy, self.h)
 
     def close(self):
-        if self.h:
-            self.L.kata_attn_destroy(self.h)
-            self.h = C.c_void_p()
+        self.h, self._native = C.c_void_p(), None
 
     def __del__(self):
         try:
@@ -261,11 +282,7 @@ class AttnContext:
     def plane_tensor(self, layer, seq, plane, nrows) -> torch.Tensor:
         """A uint8 CUDA tensor [nrows][row bytes] aliasing the plane's rows (through kata_attn_kv_plane_ptr): lets a test write rows with a
         device-side copy, as a device-resident restore would."""
-        rb = self.plane_row_bytes(plane)
-
-        class _Alias:
-            __cuda_array_interface__ = {"shape": (nrows, rb), "typestr": "|u1", "data": (self.plane_ptr(layer, seq, plane), False), "version": 3, "strides": None}
-        return torch.as_tensor(_Alias(), device=torch.device("cuda", self.device))
+        return _alias(self._native, self.plane_ptr(layer, seq, plane), (nrows, self.plane_row_bytes(plane)), "|u1", torch.device("cuda", self.device))
 
 
 def decode_static(k_rows, v_rows, seq_row0, pos_base, T, q16, gate, first_pos=0, out=None, out_dtype=torch.float32):
@@ -480,7 +497,7 @@ class PagedContext:
         self.heads, self.kv_heads, self.head_dim, self.kv_mode, self.gated, self.weights = heads, kv_heads, head_dim, kv_mode, gated, weights
         if kv_mode not in _KV_MODES:
             raise ValueError(f"kv_mode {kv_mode!r}: fp16 or int8")
-        self.planes = dict(planes or {})   # kept alive: the context works on them
+        self.planes = dict(planes or {})
         for name, t in self.planes.items():
             if name not in _PLANES:
                 raise ValueError(f"plane {name!r}: one of {_PLANES}")
@@ -495,11 +512,11 @@ class PagedContext:
         rc = L.kata_paged_create(C.byref(cfg), C.byref(self.h))
         if rc != OK:
             raise KataError(rc, "kata_paged_create failed")
+        self._native = _Native(L.kata_paged_destroy, self.h)
+        self._native.planes = self.planes   # the context works on them as long as it lives
 
     def close(self):
-        if self.h:
-            self.L.kata_paged_destroy(self.h)
-            self.h = C.c_void_p()
+        self.h, self._native = C.c_void_p(), None
 
     def __del__(self):
         try:
@@ -543,7 +560,7 @@ class PagedContext:
         return self.L.kata_pages_free_count(self.L.kata_paged_table(self.h))
 
     def plane(self, layer: int, name: str) -> torch.Tensor:
-        """A layer's plane as a tensor that aliases it: k, v [pages][page_size][kv_heads][head_dim], scales [pages][page_size][kv_heads], weight and age [pages][kv_heads][page_size]."""
+        """A layer's plane as a tensor that aliases it (and keeps the plane's memory as long as it lives, past close() too): k, v [pages][page_size][kv_heads][head_dim], scales [pages][page_size][kv_heads], weight and age [pages][kv_heads][page_size]."""
         P, S, H, D = self.n_pages, self.page_size, self.kv_heads, self.head_dim
         kv = name in ("k", "v")
         shape = (P, S, H, D) if kv else (P, S, H) if name.endswith("scale") else (P, H, S)
@@ -553,10 +570,7 @@ class PagedContext:
         if not ptr:
             raise KataError(3, f"no plane {name!r}")
         kind = ("|i1" if self.kv_mode == "int8" else "<f2") if kv else {"weight": "<f4", "age": "<i4"}.get(name, "<f2")
-
-        class _Alias:
-            __cuda_array_interface__ = {"shape": shape, "typestr": kind, "data": (ptr, False), "version": 3, "strides": None}
-        return torch.as_tensor(_Alias(), device=self.cuda)
+        return _alias(self._native, ptr, shape, kind, self.cuda)
 
     # ---- the operators
     def _at(self, what, t, n, kinds):
