@@ -95,7 +95,8 @@ int kata_attn_prep(kata_attn_ctx* ctx, int32_t layer, int32_t n, const int32_t* 
 /* No reference counterpart: kata_attn_prep with rotary positions of three axes (time, height, width), for prompts that hold images or video. The rows still go to positions pos0[b]+t
  * of the cache (what a token sees is decided by its row); only the angles take their position from d_axis_pos [n][T][3] int32 (device, the same for all layers; text tokens have one value on all
  * three axes). section[0..2], host, sum 32: how many of the 32 rotary frequencies turn by axis 0, 1, 2. interleaved 0: they lie one after the other; 1: frequency i belongs to
- * axis i % 3 while i < 3 * section[i % 3], else to axis 0. Three equal positions pos0[b]+t give kata_attn_prep's bytes. */
+ * axis i % 3 while i < 3 * section[i % 3], else to axis 0. Three equal positions pos0[b]+t give kata_attn_prep's bytes:
+ * angles are formed in fp32, as there and in the reference, off by up to 2^-23 of their size (0.007 at position 130,000; kata_paged_prep forms them exactly). */
 int kata_attn_prep_axes(kata_attn_ctx* ctx, int32_t layer, int32_t n, const int32_t* seq_ids, const int32_t* pos0, int32_t T,
                         const int32_t* d_axis_pos, const int32_t* section, int32_t interleaved,
                         const void* d_qfull, const void* d_kproj, const void* d_vproj, int32_t act_dtype,

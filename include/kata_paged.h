@@ -93,7 +93,8 @@ const kata_pages* kata_paged_table(const kata_paged_ctx* ctx);
  * (kata_attn_prep forms it in fp32, as the reference does: at position 130,000 that is 0.007 off).
  *   d_q [n][T][heads][head_dim, or 2 head_dim when gated], d_k, d_v [n][T][kv_heads][head_dim]: act_dtype; d_qnorm, d_knorm fp32 [head_dim]
  *   d_axis_pos [n][T][3] int32 (device), or NULL: all three axes are at age0[b] + t (text)
- *   age0 [n]: tokens the sequence has seen before this call, the age of its first token here; NULL: slot0
+ *   age0 [n]: tokens the sequence has seen before this call, the age of its first token here; NULL: slot0, which is right until kata_paged_evict has cut the sequence: from then on
+ *   a slot's number is not its token's age (nor its text position), and the caller says it
  *   d_q16 [n][T][heads][head_dim] fp16: the query times 1/sqrt(head_dim); d_gate [n][T][heads][head_dim] fp32, NULL when not gated (or not wanted)
  * d_q NULL appends K and V alone. With KATA_PAGED_WEIGHTS the appended slots get weight 0 and their age. */
 int kata_paged_prep(kata_paged_ctx* ctx, int32_t layer, int32_t n, const int32_t* seq_ids, const int32_t* slot0, int32_t T, const int32_t* d_axis_pos, const int32_t* age0,

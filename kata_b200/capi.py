@@ -581,7 +581,7 @@ class PagedContext:
 
     def prep(self, layer, seq_ids, slot0, T, q, k, v, qnorm, knorm, axis_pos=None, age0=None, q16=None, gate=None):
         """Norm, rotary positions and append of T tokens per sequence into slots slot0.. (kata_paged_prep). q [n][T][heads][(2) head_dim] or None, k, v [n][T][kv_heads][head_dim], axis_pos int32
-        [n][T][3] or None (text: age0 + t on every axis). Returns (q16, None, gate) as AttnContext.prep does."""
+        [n][T][3] or None (text: age0 + t on every axis). age0: tokens seen before; slot0 by default, which is right until slots of a sequence are evicted. Returns (q16, None, gate) as AttnContext.prep does."""
         ids, at0, ages, D = _ints(seq_ids), _ints(slot0), None if age0 is None else _ints(age0), self.head_dim
         n = len(ids)
         if len(at0) != n or (ages is not None and len(ages) != n):
@@ -632,5 +632,5 @@ class PagedContext:
         return src
 
     def import_rows(self, layer, seq, slot0, n_rows, src: AttnContext, src_layer, src_seq, src_pos, age0=None):
-        """Copies n_rows rows of a contiguous context into slots slot0.. (kata_paged_import)."""
+        """Copies n_rows rows of a contiguous context into slots slot0.. (kata_paged_import). age0: the first row's age; slot0 by default, which is right until slots of the sequence are evicted."""
         self._ck(self.L.kata_paged_import(self.h, layer, seq, slot0, n_rows, slot0 if age0 is None else age0, src.h, src_layer, src_seq, src_pos, self._s()))

@@ -7,7 +7,7 @@
 // ranges' partial rows joined by the last CTA of a segment (at most 8 of them) or by a combine grid. Inside a CTA four rings of a score warp and two value warps take
 // the tiles in turn; producer warps refill the rings' stages with TMA. The three kinds of warps pass from one segment into the next on their own (mbarriers for what they hand over, named barriers
 // within a kind): the producers and the score warps work on the next segment while the value warps add the rings up and write the rows. With all of them stopping at a segment's end, 32 int8
-// sequences of 300 to 32K slots took 202 us (182 now), 256 fp16 sequences of 200 slots 68 us (62). What pages change:
+// sequences of 300 to 32K slots took 202 us in short loops (182 so; in long ones the clock falls under the power limit: 191 to 216, by the GPU), 256 fp16 sequences of 200 slots 68 us (62). What pages change:
 //  - A tile is made of 16-slot groups, and a group never crosses a page (pages are powers of two from 16 slots on). The tensor map is a rank-5 view of
 //    the pool, {128-byte column block, 16 rows, column blocks, 16-row groups, KV heads}: the group is a coordinate, so one instruction
 //    brings the 16 or 32 slots of a tile wherever their page lies, in the same shared-memory order ([group][column block][16 rows][128 bytes], swizzled) for
@@ -24,7 +24,8 @@
 // for the whole segment. With the query rows as the 16 rows instead, 32 sequences of 300 to 32K int8 slots took 280 us (228 at that time).
 //
 // Precision: fp16 products, fp32 sums. The exponent carries an offset (kPShift) so that p lies high in fp16's range: it cancels in p / l and keeps
-// small p out of the subnormals. p goes into P.V in two fp16 terms (about 22 bits; int8 caches with 16-bit outputs: one term, 2^-11 relative, there the second costs time), for int8 caches times the slot's V scale in units of
+// small p out of the subnormals. p goes into P.V in two fp16 terms (about 22 bits; int8 caches with 16-bit outputs: one term, 2^-11 relative, below bf16's own step: the second
+// costs 32 ragged sequences 201 us instead of 191, with two tokens 264 instead of 244, and 18 of 15,000 slots with heads of 128 106 instead of 102), for int8 caches times the slot's V scale in units of
 // a power of two above the largest V scale of the tile: O and alpha carry the units from tile to tile, so small values keep as many bits as large ones (with the bare scale, whose products sank into fp16's subnormals, outputs
 // were off by 1e-5 at V scales of 1e-3 and by 1 % at 1e-6). What is lost lies below 2^-40 of the row's heaviest p times the tile's largest scale. int8 codes are taken
 // without the 1152 bias of the contiguous kernel (whose subtraction costs some ten bits), and a tile's P.V is formed in fresh accumulators and added to O with a rounded fma (the matrix
@@ -778,7 +779,7 @@ int split_paged_tiles(PagedPlan& p, int tile_keys, int sm_count) {
         p.cut[p.n_ctas] = total;
     } else {
         // A segment costs a CTA more than its tiles: its rows are joined and written, the next one's query staged, some 3 us beside 0.37 us a tile. Many short segments would pile up in a few CTAs
-        // (32 int8 sequences of 300 to 32K slots, sorted by length: 218 us, 182 like this): each counts as kPad tiles more, where the ranges are long enough for that. A cut that falls within kSnap tiles of an
+        // (32 int8 sequences of 300 to 32K slots, sorted by length, in short loops: 218 us, 182 like this): each counts as kPad tiles more, where the ranges are long enough for that. A cut that falls within kSnap tiles of an
         // end of a segment moves there: less than what the second piece would cost.
         p.n_ctas = std::max(1, std::min(sm_count, total));
         const int pad = total >= (int64_t)sm_count * 4 * kPad ? kPad : 0, snap = pad ? kSnap : 0; const int64_t places = total + (int64_t)n_seg * pad;
