@@ -155,8 +155,10 @@ __device__ __forceinline__ void paged_scores(const uint32_t q_sm, const uint32_t
 // Online softmax state of query rows nr * 8 + 2 * t4 + {0, 1}: maximum (log2 units) and this lane's share of the sum
 template <int NR> struct RowsState { float m[NR][2], l[NR][2]; };
 
-// pr = 2^SHIFT * exp(s - m) in place of s; the state and the rescale factors brought up to date.
-template <int NK, int NR, int SHIFT>
+// pr = 2^SHIFT * 2^(s - m) in place of s; the state and the rescale factors brought up to date. LOG2: s is in log2 units already, so that no score passes the maximum (s - (m - SHIFT) may round up to 16, where P's
+// scale below 1 keeps it within fp16). Else the product with log2 e is fused with the subtraction; above kRoundedMax it and the rounded maximum can be whole units apart, P would leave fp16's range, and it is rounded too.
+constexpr float kRoundedMax = 0x1p22f;
+template <int NK, int NR, int SHIFT, bool LOG2>
 __device__ __forceinline__ void paged_softmax(float (&s)[NK][NR][4], RowsState<NR>& st, float (&al)[NR][2]) {
 #pragma unroll
     for (int nr = 0; nr < NR; nr++)
@@ -165,14 +167,19 @@ __device__ __forceinline__ void paged_softmax(float (&s)[NK][NR][4], RowsState<N
             float mx = -INFINITY;
 #pragma unroll
             for (int sb = 0; sb < NK; sb++) mx = fmaxf(mx, fmaxf(s[sb][nr][e], s[sb][nr][2 + e]));
-            mx *= kLog2e;
+            if (!LOG2) mx *= kLog2e;
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8)); mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             const float mn = fmaxf(st.m[nr][e], mx), sub = (mn == -INFINITY) ? 0.0f : mn - SHIFT;
             al[nr][e] = (mn == -INFINITY) ? 1.0f : ex2(st.m[nr][e] - mn); st.m[nr][e] = mn;
-            float sum = 0.0f;
+            float sum = 0.0f, scale = kLog2e, add = -sub;
+            if (!LOG2 && fabsf(mn) > kRoundedMax && fabsf(mn) < INFINITY) {
+#pragma unroll
+                for (int sb = 0; sb < NK; sb++) { s[sb][nr][e] = __fmul_rn(s[sb][nr][e], kLog2e) - mn; s[sb][nr][2 + e] = __fmul_rn(s[sb][nr][2 + e], kLog2e) - mn; }
+                scale = 1.0f; add = SHIFT;
+            }
 #pragma unroll
             for (int sb = 0; sb < NK; sb++) {
-                s[sb][nr][e] = ex2(fmaf(s[sb][nr][e], kLog2e, -sub)); s[sb][nr][2 + e] = ex2(fmaf(s[sb][nr][2 + e], kLog2e, -sub));
+                s[sb][nr][e] = ex2(LOG2 ? s[sb][nr][e] - sub : fmaf(s[sb][nr][e], scale, add)); s[sb][nr][2 + e] = ex2(LOG2 ? s[sb][nr][2 + e] - sub : fmaf(s[sb][nr][2 + e], scale, add));
                 sum += s[sb][nr][e] + s[sb][nr][2 + e];
             }
             st.l[nr][e] = st.l[nr][e] * al[nr][e] + sum;
@@ -500,7 +507,7 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         if (K8) sc[sb][e] = *reinterpret_cast<const uint32_t*>(smem + G::kOffScale + (ring * kStages + stg) * kTile * 4 + (16 * sb + 8 * e + g) * 4);
-                        ks[sb][e] = K8 ? __half2float(__ushort_as_half((unsigned short)sc[sb][e])) : 1.0f;
+                        ks[sb][e] = K8 ? __half2float(__ushort_as_half((unsigned short)sc[sb][e])) * kLog2e : 1.0f;   // int8: scores in log2 units
                     }
                 float s[NK][NR][4], al[NR][2];
                 paged_scores<HD, K8, NR>(sm_base, ring_stage0 + stg * G::kStageBytes, qf, ks, lane, s);
@@ -535,7 +542,7 @@ __global__ void __launch_bounds__(PGeo<HD, K8, NR>::kThreads, 1) paged_decode_ke
 #pragma unroll
                             for (int e = 0; e < 2; e++) *reinterpret_cast<float2*>(st + (16 * sb + 8 * e) * srow + nr * 8) = make_float2(s[sb][nr][2 * e], s[sb][nr][2 * e + 1]);
                 }
-                paged_softmax<NK, NR, G::kPShift>(s, ss, al);
+                paged_softmax<NK, NR, G::kPShift, K8>(s, ss, al);
                 if (K8) {   // P holds p times the V scale in units of 2^(exponent of the tile's largest + 1), so that it fills fp16's range whatever the size of the values; O follows from tile to tile by alpha
                     float vs[NK][2], top = 0.0f;
 #pragma unroll
@@ -730,12 +737,12 @@ __global__ void __launch_bounds__(1024) paged_combine_kernel(const __grid_consta
     paged_emit(p, o, b, kvh, r, d, at, paged_gate(o, at), M, L, A0, A1);
 }
 
-// weight[kv head][slot] += sum over the rows of 2^(s * log2 e - m + shift) / l: the slot's final probabilities, from the scores the decode kernel
+// weight[kv head][slot] += sum over the rows of 2^(s * log2 e - m + shift) / l (int8: s is in log2 units): the slot's final probabilities, from the scores the decode kernel
 // kept and the joined (m, 1 / l). A thread per (slot, KV head) in the order of the tile list: 32 (or 64) contiguous bytes per thread, nothing shared, no atomics. All of a thread's requests are
 // under way before the first is used (107K slots x 4 heads: 7.9 us, 10.3 with a loop over the rows).
 template <int ROWS>   // 8 or 16 stored rows
 __global__ void __launch_bounds__(256) paged_weight_kernel(const __grid_constant__ PagedPlan p, const int32_t* __restrict__ tables, const float* __restrict__ scores, const float* __restrict__ fin_ml,
-                                                           float* __restrict__ weight /* the layer's plane [page][kv head][slot] */, const int tile_shift, const float shift) {
+                                                           float* __restrict__ weight /* the layer's plane [page][kv head][slot] */, const int tile_shift, const float shift, const bool log2) {
     const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x; const int tile = (int)(idx >> tile_shift);
     int lo = 0, hi = p.n - 1;
     while (lo < hi) { const int mid = (lo + hi + 1) >> 1; if (p.tile_start[mid] <= tile) lo = mid; else hi = mid - 1; }
@@ -754,7 +761,7 @@ __global__ void __launch_bounds__(256) paged_weight_kernel(const __grid_constant
 #pragma unroll
     for (int r = 0; r < ROWS; r++) {
         const float x = r % 4 == 0 ? v[r / 4].x : r % 4 == 1 ? v[r / 4].y : r % 4 == 2 ? v[r / 4].z : v[r / 4].w, m = r & 1 ? ml[r / 2].z : ml[r / 2].x, inv = r & 1 ? ml[r / 2].w : ml[r / 2].y;
-        if (r < rows && x != -INFINITY) sum += ex2(fmaf(x, kLog2e, shift - m)) * inv;   // a masked slot adds nothing (its row may have no maximum at all)
+        if (r < rows && x != -INFINITY) sum += ex2(log2 ? x - (m - shift) : fabsf(m) > kRoundedMax ? (__fmul_rn(x, kLog2e) - m) + shift : fmaf(x, kLog2e, shift - m)) * inv;   // as the decode kernel formed it (log2: int8); a masked slot adds nothing (its row may have no maximum at all)
     }
     *at = before + sum;
 }
@@ -848,7 +855,7 @@ cudaError_t launch_paged_decode(PagedCtx& c, int layer, int n, const int32_t* se
         if (accumulate) {
             const int64_t keys = (int64_t)p.tile_start[n] * tile_keys;
             e = launch_pdl(c.group * p.T > 8 ? paged_weight_kernel<16> : paged_weight_kernel<8>, dim3((unsigned)((keys + 255) / 256)), dim3(256), 0, s, p, (const int32_t*)c.d_table, (const float*)c.scores, (const float*)c.fin_ml,
-                           (float*)c.layer_plane(KATA_PAGED_WEIGHT, layer), tile_keys == 16 ? 4 : tile_keys == 32 ? 5 : 6, c.int8() ? (float)PGeo<256, true, 1>::kPShift : (float)PGeo<256, false, 1>::kPShift);
+                           (float*)c.layer_plane(KATA_PAGED_WEIGHT, layer), tile_keys == 16 ? 4 : tile_keys == 32 ? 5 : 6, (float)PGeo<256, true, 1>::kPShift, c.int8());
             if (e != cudaSuccess) return e;
             c.launches++;
         }

@@ -2,11 +2,11 @@
 largest, and long int8 caches head by head; each against a plain evaluation in 64 bits.
 
 Elementwise bounds are relative to A = sum_j p_j |v_j| / l, the size of the terms an output is made of:
- - scores: q, codes and K scales are chosen so that every partial sum is exact; the exponent's argument (|x| < 32) is rounded twice, 2 * 32 * 2^-24 * ln 2, and ex2 is off by 2^-22. Both
-   occur in numerator and denominator: 2 * (2.7e-6 + 2.4e-7) = 5.9e-6
+ - scores: q, codes and K scales are chosen so that every partial sum is exact; the exponent's argument (|x| < 32) is rounded three times, 3 * 32 * 2^-24 * ln 2, and ex2 is off by 2^-22. Both
+   occur in numerator and denominator: 2 * (4.0e-6 + 2.4e-7) = 8.4e-6
  - p times the V scale in two fp16 terms: 2^-22, or 2^-25 of a number that is carried as 2^15 p v / (at most twice the tile's largest scale): 2^-40 of that scale a slot; in one term 2^-11 instead of 2^-22
  - products: up to 8 chained matrix instructions per tile, 2 * 2^-23 each; then one rounding a tile and four joins: 1,000 slots are below 64 tiles, 2^-18 in all
- together 5.9e-6 + 2.4e-7 + 1.9e-6 + 3.8e-6 < 2^-16; outputs add half a step of their type."""
+ together 8.4e-6 + 2.4e-7 + 1.9e-6 + 3.8e-6 < 2^-16; outputs add half a step of their type."""
 import math
 
 import pytest
